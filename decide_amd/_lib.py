@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_uint16, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_uint16, c_uint32, c_uint64, c_void_p
 
 # DH_LIB names another build of the same library (the sanitizer builds of decide_amd/csrc/Makefile); unset, the
 # in-tree library is the one loaded.
@@ -67,6 +67,31 @@ class DhAnswer(ctypes.Structure):
 
     _fields_ = [("row", c_uint32), ("ncand", c_uint32), ("cand", POINTER(c_uint32))]
 
+
+class DhKv8Cache(ctypes.Structure):
+    """``dh_kv8_cache`` (include/decide_hip.h)."""
+
+    _fields_ = [("pool", c_void_p), ("pages", c_uint32), ("layers", c_uint32), ("kv_heads", c_uint32),
+                ("head_dim", c_uint32), ("format", c_uint32)]
+
+
+class DhKv8Batch(ctypes.Structure):
+    """``dh_kv8_batch`` (include/decide_hip.h)."""
+
+    _fields_ = [("table", c_void_p), ("row0", c_void_p), ("qpos", c_void_p), ("ld_table", c_uint32),
+                ("seqs", c_uint32), ("rows", c_uint32)]
+
+
+class DhRopeSpec(ctypes.Structure):
+    """``dh_rope_spec`` (include/decide_hip.h)."""
+
+    _fields_ = [("inv_freq", c_void_p), ("norm_w", c_void_p), ("head_dim", c_uint32), ("rot", c_uint32),
+                ("layout", c_uint32), ("add_one", c_uint32), ("eps", c_float), ("amp", c_float)]
+
+
+DH_KV8_PAGE = 64
+DH_KV8_BLOCK = 16
+DH_KV8_NO_POSITION = 0xFFFFFFFF
 
 DH_FORWARD_NO_PRUNE = 1
 DH_LOGITS_FULL = 1
@@ -187,6 +212,39 @@ PROTOTYPES = {
     "dh_state_boundary": (
         c_int, [POINTER(c_uint32), c_uint32, c_uint32, POINTER(c_uint32), c_uint32, c_uint32, POINTER(c_uint32),
                 POINTER(c_int)]),
+    "dh_kv8_page_bytes": (c_uint64, [c_uint32, c_uint32]),
+    "dh_rope": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_uint32, c_uint32, c_void_p, c_uint32, c_uint32, c_void_p, c_uint32, c_uint32,
+         POINTER(DhRopeSpec)],
+    ),
+    "dh_rope_freqs": (
+        c_int,
+        [c_uint32, c_double, c_uint32, c_double, c_double, c_double, c_uint32, POINTER(c_float), POINTER(c_float)],
+    ),
+    "dh_kv8_append": (
+        c_int,
+        [c_void_p, c_void_p, POINTER(DhKv8Cache), c_uint32, POINTER(DhKv8Batch), c_void_p, c_uint32, c_void_p, c_uint32,
+         c_uint32, POINTER(DhRopeSpec)],
+    ),
+    "dh_kv8_attention": (
+        c_int,
+        [c_void_p, c_void_p, POINTER(DhKv8Cache), c_uint32, POINTER(DhKv8Batch), c_void_p, c_uint32, c_uint32, c_float,
+         c_void_p, c_uint32, c_void_p, c_uint32, c_uint32],
+    ),
+    "dh_kv8_attention_ws": (
+        c_int, [c_void_p, c_void_p, POINTER(DhKv8Cache), c_uint32, c_uint32, c_uint32, c_uint32]),
+    "dh_kv8_copy_pages": (c_int, [c_void_p, c_void_p, POINTER(DhKv8Cache), c_void_p, c_void_p, c_uint32]),
+    "dh_pages_create": (c_int, [c_uint32, c_uint32, POINTER(c_void_p)]),
+    "dh_pages_destroy": (None, [c_void_p]),
+    "dh_pages_resize": (
+        c_int, [c_void_p, c_uint32, c_uint64, POINTER(c_uint32), POINTER(c_uint32), POINTER(c_uint32)]),
+    "dh_pages_fork": (c_int, [c_void_p, c_uint32, c_uint32, c_uint64]),
+    "dh_pages_compact": (c_int, [c_void_p, POINTER(c_uint32), POINTER(c_uint32), c_uint32, POINTER(c_uint32)]),
+    "dh_pages_table": (
+        c_int, [c_void_p, c_uint32, POINTER(c_uint64), POINTER(c_uint32), c_uint32, POINTER(c_uint32)]),
+    "dh_pages_free": (c_uint32, [c_void_p]),
+    "dh_pages_refs": (c_uint32, [c_void_p, c_uint32]),
 }
 
 _lib = None

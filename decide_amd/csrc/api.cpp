@@ -506,9 +506,10 @@ int dh_warm_up(dh_ctx* ctx, void* stream, uint32_t max_m) {
   // streaming kernel (M = 16, N = 32, K = 128) into scratch.
   void* scratch = nullptr;
   const size_t xb = 16 * 128 * 2, wb = 512 * 64 * 2, yb = 16 * 512 * 4;
-  hipError_t e = hipMalloc(&scratch, xb + wb + yb);
+  const size_t gemm_bytes = (xb + wb + yb + 127) / 128 * 128;
+  hipError_t e = hipMalloc(&scratch, gemm_bytes + kv8_warm_bytes());
   if (e != hipSuccess) return fail(DH_ENOMEM, "dh_warm_up: %s", hipGetErrorString(e));
-  e = hipMemsetAsync(scratch, 0, xb + wb + yb, s);
+  e = hipMemsetAsync(scratch, 0, gemm_bytes + kv8_warm_bytes(), s);
   int rc = hip_status(e, "dh_warm_up memset");
   char* base = (char*)scratch;
   for (int v = 0; v < dh::variant_count() && rc == DH_OK; ++v) {
@@ -526,6 +527,7 @@ int dh_warm_up(dh_ctx* ctx, void* stream, uint32_t max_m) {
     dh_gemm_member mem{base + xb, base + xb + wb, 128, (uint32_t)vi.bn(), (uint32_t)vi.bn(), DH_EPI_STORE_F32};
     rc = launch_plan(ctx, s, dh::plan_make(0, 2, 8, vi.bn(), 128), base, 128, 8, 128, &mem, 1);
   }
+  if (rc == DH_OK) rc = kv8_warm(ctx, s, base + gemm_bytes);
   if (rc == DH_OK) {
     e = hipStreamSynchronize(s);
     rc = hip_status(e, "dh_warm_up sync");

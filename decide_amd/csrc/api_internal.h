@@ -47,7 +47,8 @@ constexpr int kMaxTileVariants = 24;
 enum : int {
   kKidReduce = kMaxTileVariants, kKidReference, kKidGather32, kKidGather16, kKidHead, kKidNorm, kKidFill,
   kKidConv, kKidConvState, kKidDelta, kKidGNorm, kKidQRope, kKidKVRope, kKidAttn, kKidEmbed, kKidFillAny,
-  kKidDeltaChunk, kKidStream, kKidAttnCombine, kKidConvDelta, kKidAddNorm, kKidDeltaBlock, kKidCount
+  kKidDeltaChunk, kKidStream, kKidAttnCombine, kKidConvDelta, kKidAddNorm, kKidDeltaBlock,
+  kKidRope, kKidKv8Append, kKidKv8Attn, kKidKv8Combine, kKidKv8Copy, kKidCount
 };
 static_assert(kKidCount <= 64, "kernel ids must fit dh_ctx::used");
 
@@ -72,5 +73,9 @@ bool forced_plan(const dh_ctx* c, int* variant, uint32_t* splits);
 // forward knows it (the chunk's last position + 1).
 int attention_run(dh_ctx* ctx, void* stream, const uint16_t* q, const uint16_t* kc, const uint16_t* vc,
                   const float* pq, const uint32_t* qpos, uint16_t* y, uint32_t rows, uint32_t ldq, uint32_t npos);
+
+// Launches every kernel of the 8-bit cache once on tiny inputs (dh_warm_up): `mem` holds kv8_warm_bytes() zeroed bytes.
+size_t kv8_warm_bytes();
+int kv8_warm(dh_ctx* ctx, hipStream_t s, void* mem);
 
 }  // namespace dh_api

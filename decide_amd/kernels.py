@@ -21,7 +21,7 @@ from __future__ import annotations
 
 import ctypes
 import enum
-from typing import Iterable, Sequence, Tuple, Union
+from typing import Iterable, Optional, Sequence, Tuple, Union
 
 from . import _lib
 
@@ -267,6 +267,32 @@ class GNorm:
                                              addr(y), t, ldz))
 
 
+DTYPE_CODES = {"f16": 0, "bf16": 1, "f32": 2}  # element types, as fill_normal's
+ROPE_LAYOUTS = {"half": 0, "interleaved": 1}
+ROPE_SCALINGS = {"plain": 0, "linear": 1, "base": 2, "parts": 3}
+KV8_FORMATS = {"e4m3": 0, "int8": 1}
+
+
+def rope_freqs(rot: int, base: float, scaling: str = "plain", factor: float = 1.0, low: float = 1.0, high: float = 32.0,
+               trained_len: int = 1) -> Tuple[list, float]:
+    """``(inv_freq, amp)`` of a rotary embedding whose positions are stretched by ``factor`` (host; dh_rope_freqs)."""
+    lib = _lib.load()
+    f, amp = (ctypes.c_float * max(rot // 2, 1))(), ctypes.c_float()
+    _call(lib.dh_rope_freqs(rot, base, ROPE_SCALINGS[scaling], factor, low, high, trained_len, f, ctypes.byref(amp)))
+    return list(f), amp.value
+
+
+class RopeSpec:
+    """``dh_rope_spec``: pairs, angles and the norm before them. Keeps its buffers alive."""
+
+    def __init__(self, inv_freq: Arg, head_dim: int, rot: int, layout: str = "half", amp: float = 1.0,
+                 norm_w: Optional[Arg] = None, add_one: bool = True, eps: float = 1e-6):
+        self.keep = (inv_freq, norm_w)
+        self.c = _lib.DhRopeSpec(addr(inv_freq), None if norm_w is None else addr(norm_w), head_dim, rot,
+                                 ROPE_LAYOUTS[layout], 1 if add_one else 0, eps, amp)
+        self.ref = ctypes.byref(self.c)
+
+
 class Rope:
     """decide's ``Rope`` (kernels/rope.rs:16-54)."""
 
@@ -285,6 +311,13 @@ class Rope:
                                        addr(kc), addr(vc), rows, ldkv, kcol, vcol, pos0))
 
 
+    def rope(self, stream: int, x: Arg, ldx: int, x_dtype: str, y: Arg, ldy: int, y_dtype: str, pos: Arg, rows: int,
+             heads: int, spec: RopeSpec) -> None:
+        """y[r, h] = rope(norm(x[r, h]), pos[r]) in any layout of ``RopeSpec``; decide has only ``q_norm_rope``'s."""
+        _call(self.lib.dh_rope(self.ctx.handle, stream, addr(x), ldx, DTYPE_CODES[x_dtype], addr(y), ldy,
+                               DTYPE_CODES[y_dtype], addr(pos), rows, heads, spec.ref))
+
+
 class Attn:
     """decide's ``Attn`` (kernels/attn.rs:44-125)."""
 
@@ -296,6 +329,113 @@ class Attn:
                   ldq: int) -> None:
         _call(self.lib.dh_attention(self.ctx.handle, ctypes.c_void_p(stream), addr(q), addr(kc), addr(vc), addr(pq),
                                     addr(qpos), addr(y), rows, ldq))
+
+
+def kv8_page_bytes(kv_heads: int, head_dim: int) -> int:
+    """Bytes of one page (64 tokens) of one layer of an 8-bit cache."""
+    return int(_lib.load().dh_kv8_page_bytes(kv_heads, head_dim))
+
+
+class Kv8Cache:
+    """``dh_kv8_cache``: a pool of pages, uint8 [layers][pages][kv8_page_bytes]. Keeps the pool's buffer alive."""
+
+    def __init__(self, pool: Arg, pages: int, layers: int, kv_heads: int, head_dim: int, format: str = "e4m3"):
+        self.keep = pool
+        self.c = _lib.DhKv8Cache(addr(pool), pages, layers, kv_heads, head_dim, KV8_FORMATS[format])
+        self.ref = ctypes.byref(self.c)
+
+
+class Kv8Batch:
+    """``dh_kv8_batch``: the rows of a call, their positions, their sequences' page tables. Keeps the buffers alive."""
+
+    def __init__(self, table: Arg, ld_table: int, row0: Arg, qpos: Arg, seqs: int, rows: int):
+        self.keep = (table, row0, qpos)
+        self.c = _lib.DhKv8Batch(addr(table), addr(row0), addr(qpos), ld_table, seqs, rows)
+        self.ref = ctypes.byref(self.c)
+
+
+class Kv8:
+    """The 8-bit paged key/value cache (decide's caches are fp16 and contiguous: kernels/rope.rs:39-54,
+    kernels/attn.rs:80-125)."""
+
+    def __init__(self, ctx: Context):
+        self.ctx = ctx
+        self.lib = ctx.lib
+
+    def append(self, stream: int, cache: Kv8Cache, layer: int, batch: Kv8Batch, k: Arg, ldk: int, v: Arg, ldv: int,
+               dtype: str, rope: Optional[RopeSpec] = None) -> None:
+        """Codes K (normed and turned first, with ``rope``) and V rows into their sequences' pages."""
+        _call(self.lib.dh_kv8_append(self.ctx.handle, stream, cache.ref, layer, batch.ref, addr(k), ldk, addr(v), ldv,
+                                     DTYPE_CODES[dtype], None if rope is None else rope.ref))
+
+    def attention(self, stream: int, cache: Kv8Cache, layer: int, batch: Kv8Batch, q: Arg, ldq: int, heads: int,
+                  scale: float, y: Arg, ldy: int, max_tokens: int, gate: Optional[Arg] = None, ldg: int = 0) -> None:
+        """y = softmax(scale q·kᵀ)·v (⊙ σ(gate)) of each row over its sequence's tokens up to its position."""
+        _call(self.lib.dh_kv8_attention(self.ctx.handle, stream, cache.ref, layer, batch.ref, addr(q), ldq, heads, scale,
+                                        None if gate is None else addr(gate), ldg, addr(y), ldy, max_tokens))
+
+    def attention_ws(self, stream: int, cache: Kv8Cache, rows: int, seqs: int, heads: int, max_tokens: int) -> None:
+        """Sizes ``stream``'s workspace for ``attention`` calls of these sizes (before a capture)."""
+        _call(self.lib.dh_kv8_attention_ws(self.ctx.handle, stream, cache.ref, rows, seqs, heads, max_tokens))
+
+    def copy_pages(self, stream: int, cache: Kv8Cache, src: Arg, dst: Arg, n: int) -> None:
+        """Page src[i] → dst[i] in every layer, i < n (device arrays of page ids)."""
+        _call(self.lib.dh_kv8_copy_pages(self.ctx.handle, stream, cache.ref, addr(src), addr(dst), n))
+
+
+class Pages:
+    """``dh_pages``: which pages which sequence holds, in host memory: reference counts, forks, copy on write."""
+
+    def __init__(self, pages: int, max_seqs: int):
+        self.lib = _lib.load()
+        self.pages = pages
+        h = ctypes.c_void_p()
+        _call(self.lib.dh_pages_create(pages, max_seqs, ctypes.byref(h)))
+        self.handle = h
+
+    def resize(self, seq: int, tokens: int) -> Optional[Tuple[int, int]]:
+        """Make ``seq`` hold ``tokens`` tokens; the (src, dst) page copy to make before an append, or None."""
+        s, d, n = ctypes.c_uint32(), ctypes.c_uint32(), ctypes.c_uint32()
+        _call(self.lib.dh_pages_resize(self.handle, seq, tokens, ctypes.byref(s), ctypes.byref(d), ctypes.byref(n)))
+        return (s.value, d.value) if n.value else None
+
+    def fork(self, src: int, dst: int, tokens: int) -> None:
+        """``dst`` (empty) shares the pages of ``src``'s first ``tokens`` tokens."""
+        _call(self.lib.dh_pages_fork(self.handle, src, dst, tokens))
+
+    def compact(self) -> list:
+        """Move held pages to the lowest ids: the (src, dst) copies to make."""
+        n = ctypes.c_uint32()
+        src, dst = (ctypes.c_uint32 * self.pages)(), (ctypes.c_uint32 * self.pages)()
+        _call(self.lib.dh_pages_compact(self.handle, src, dst, self.pages, ctypes.byref(n)))
+        return [(src[i], dst[i]) for i in range(n.value)]
+
+    def table(self, seq: int) -> Tuple[int, list]:
+        """(tokens, page ids) of a sequence."""
+        tokens, n = ctypes.c_uint64(), ctypes.c_uint32()
+        _call(self.lib.dh_pages_table(self.handle, seq, ctypes.byref(tokens), None, 0, ctypes.byref(n)))
+        ids = (ctypes.c_uint32 * max(n.value, 1))()
+        _call(self.lib.dh_pages_table(self.handle, seq, ctypes.byref(tokens), ids, n.value, ctypes.byref(n)))
+        return int(tokens.value), list(ids[:n.value])
+
+    def free(self) -> int:
+        """Pages that no sequence holds."""
+        return int(self.lib.dh_pages_free(self.handle))
+
+    def refs(self, page: int) -> int:
+        """Sequences that hold ``page``."""
+        return int(self.lib.dh_pages_refs(self.handle, page))
+
+    def close(self) -> None:
+        if self.handle:
+            self.lib.dh_pages_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):  # pragma: no cover - interpreter shutdown order
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 def fill_normal(ctx: Context, stream: int, out: Arg, n: int, seed: int, mean: float, std: float, dtype: str) -> None:
@@ -323,3 +463,4 @@ class Kernels:
         self.gnorm = GNorm(self.ctx)
         self.rope = Rope(self.ctx)
         self.attn = Attn(self.ctx)
+        self.kv8 = Kv8(self.ctx)

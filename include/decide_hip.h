@@ -502,6 +502,183 @@ int dh_model_set_state_marker(dh_model* model, const uint32_t* marker, uint32_t 
 int dh_state_boundary(const uint32_t* ids, uint32_t len, uint32_t prefix, const uint32_t* marker, uint32_t marker_len,
                       uint32_t limit, uint32_t* boundary, int* found);
 
+/* ======================================================================
+ * The 8-bit paged key/value cache: rotary positions, the append that codes
+ * key and value rows into pages, the attention that reads them, and the
+ * copying, sharing and moving of pages. decide has no counterpart: its caches
+ * are fp16 and contiguous, one per request (kernels/rope.rs:39-54,
+ * kernels/attn.rs:80-125), and a state is copied whole
+ * (forward.rs:641-675). Here many sequences share the pages of the
+ * prefix that they have in common, and a token takes half the bytes.
+ *
+ * A cache is a pool of pages, [layers][pages] records of dh_kv8_page_bytes()
+ * each. A page holds DH_KV8_PAGE tokens of every kv head:
+ *   K codes  [kv_heads][DH_KV8_PAGE][head_dim]   (one byte each)
+ *   V codes  [kv_heads][head_dim][DH_KV8_PAGE]   (tokens innermost)
+ *   scales   [kv_heads][2][4] float              (K's, V's; one for DH_KV8_BLOCK tokens)
+ * and padding to a multiple of 128 bytes. A value is code x scale:
+ *   DH_KV8_E4M3  the byte is an OCP e4m3 number (never its NaN), the scale the smallest power of two
+ *                that brings the block's largest magnitude to at most 448;
+ *   DH_KV8_INT8  the byte b stands for b - 128 (-127..127), the scale is the largest magnitude x 1/127 (in fp32).
+ * Scales are at least 2^-100. A block (16 tokens of one head) that was given a
+ * value that is not finite has a NaN scale: all of its values are NaN.
+ * ====================================================================== */
+#define DH_KV8_PAGE 64u
+#define DH_KV8_BLOCK 16u
+#define DH_KV8_E4M3 0u
+#define DH_KV8_INT8 1u
+
+typedef struct dh_kv8_cache {
+  void* pool;         /* device memory, layers * pages * dh_kv8_page_bytes() bytes, 128-byte aligned */
+  uint32_t pages;     /* pages of one layer */
+  uint32_t layers;
+  uint32_t kv_heads;  /* 1 .. 1024 */
+  uint32_t head_dim;  /* 64, 128 or 256 */
+  uint32_t format;    /* DH_KV8_E4M3 or DH_KV8_INT8 */
+} dh_kv8_cache;
+
+/* Bytes of one page of one layer (0 for a head_dim or kv_heads out of range). */
+uint64_t dh_kv8_page_bytes(uint32_t kv_heads, uint32_t head_dim);
+
+/* The rows of one call and the sequences they belong to; device arrays.
+ * Rows row0[s] .. row0[s + 1] - 1 are sequence s's; row0 does not decrease,
+ * and entries past `rows` count as `rows`. Rows before row0[0] or from
+ * row0[seqs] on belong to none: nothing reads them or writes their outputs.
+ * Token t of sequence s lies in page table[s * ld_table + t / DH_KV8_PAGE];
+ * the same page may stand in several tables. */
+#define DH_KV8_NO_POSITION 0xffffffffu
+typedef struct dh_kv8_batch {
+  const uint32_t* table; /* [seqs][ld_table] page ids */
+  const uint32_t* row0;  /* [seqs + 1] */
+  const uint32_t* qpos;  /* [rows] each row's position in its sequence, or DH_KV8_NO_POSITION */
+  uint32_t ld_table;     /* entries of a table row */
+  uint32_t seqs;
+  uint32_t rows;         /* rows that the arrays and matrices hold (the launch is sized by it) */
+} dh_kv8_batch;
+
+/* A rotary embedding. Element pairs (i, i + rot / 2) (DH_ROPE_HALF) or
+ * (2i, 2i + 1) (DH_ROPE_INTERLEAVED), i < rot / 2, turn by the angle
+ * position * inv_freq[i], formed and reduced in 64 bits, with cos and sin
+ * multiplied by `amp`; elements from rot on pass through. With norm_w, each
+ * head is first RMS-normed over its head_dim elements and multiplied by w
+ * (add_one 0) or 1 + w. */
+#define DH_ROPE_HALF 0u
+#define DH_ROPE_INTERLEAVED 1u
+typedef struct dh_rope_spec {
+  const float* inv_freq; /* device [rot / 2] */
+  const float* norm_w;   /* device [head_dim], or NULL: no norm */
+  uint32_t head_dim;     /* a multiple of 4, 4 .. 256 */
+  uint32_t rot;          /* even, 2 .. head_dim */
+  uint32_t layout;       /* DH_ROPE_* */
+  uint32_t add_one;
+  float eps;             /* > 0 with norm_w */
+  float amp;             /* finite */
+} dh_rope_spec;
+
+/* y[r, h] = rope(norm(x[r, h]), pos[r]) for `heads` heads of spec->head_dim
+ * elements, head h at column h * head_dim of rows of stride ldx and ldy
+ * (elements). x_dtype and y_dtype: 0 fp16, 1 bf16, 2 fp32; arithmetic fp32.
+ * y may be x where dtypes and strides agree. Contract: strides cover the heads
+ * and are multiples of 4; x and y aligned to 4 of their elements; norm_w to
+ * 16 bytes. pos: device u32 [rows], every value a position.
+ * (dh_q_norm_rope is this with decide's layout: 16 heads of 256, 64 of them
+ * rotated as halves, fp32 in, fp16 out, and its angle an fp32 product.) */
+int dh_rope(dh_ctx* ctx, void* stream, const void* x, uint32_t ldx, uint32_t x_dtype, void* y, uint32_t ldy,
+            uint32_t y_dtype, const uint32_t* pos, uint32_t rows, uint32_t heads, const dh_rope_spec* spec);
+
+/* inv_freq[i] (host, [rot / 2]) and the amplitude for positions stretched by
+ * `factor` (>= 1), from f_i = base^(-2i / rot):
+ *   DH_ROPE_PLAIN   f_i (factor is not used);
+ *   DH_ROPE_LINEAR  f_i / factor: positions squeezed into the trained range;
+ *   DH_ROPE_BASE    base * factor^(rot / (rot - 2)) in place of base (rot > 2): the slowest pair squeezed by factor, the
+ *                   fastest not at all;
+ *   DH_ROPE_PARTS   f_i where pair i turns at least `high` times within trained_len positions, f_i / factor
+ *                   where it turns at most `low` times, linear in the number of turns between; amplitude
+ *                   0.1 ln(factor) + 1 (1 for the other kinds).
+ * low, high and trained_len are read by DH_ROPE_PARTS only. Computed in 64 bits. */
+#define DH_ROPE_PLAIN 0u
+#define DH_ROPE_LINEAR 1u
+#define DH_ROPE_BASE 2u
+#define DH_ROPE_PARTS 3u
+int dh_rope_freqs(uint32_t rot, double base, uint32_t kind, double factor, double low, double high,
+                  uint32_t trained_len, float* inv_freq, float* amp);
+
+/* Stores K and V rows at their sequences' ends: row r0 + i of sequence s, whose
+ * first row in the batch is r0, becomes token qpos[r0] + i (the rows of a
+ * sequence are consecutive tokens; later entries of qpos are not read). k and
+ * v: kv_heads heads of head_dim elements, dtype as dh_rope's, row strides ldk
+ * and ldv. With `rope` (head_dim as the cache's), each key is normed and
+ * turned at its token's position, in 64 bits, and rounded to fp32 before it is
+ * coded; without, keys are coded as they are. Values always are.
+ * The call ends the sequence after its last row: a block that it starts within
+ * keeps its earlier tokens (coded again where its scale grows; the scale never
+ * shrinks while tokens stay), and whatever the block of the last row held
+ * behind that row is cleared. A page that another sequence's table also holds
+ * changes for that one too: copy it first (dh_kv8_copy_pages).
+ * A token whose page id is not below cache->pages, or whose table entry would
+ * lie past ld_table, is not stored; nor is a sequence whose first row has no
+ * position. Contract: as dh_rope for k and v. */
+int dh_kv8_append(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, uint32_t layer, const dh_kv8_batch* batch,
+                  const void* k, uint32_t ldk, const void* v, uint32_t ldv, uint32_t dtype, const dh_rope_spec* rope);
+
+/* y[r, h] = softmax_t(scale * q[r, h] . K[t, g]) . V[t, g] (x sigmoid(gate[r, h])),
+ * over tokens t = 0 ..= qpos[r] of row r's sequence, kv head g = h / (heads /
+ * kv_heads); a row without a position sees no token and its y is zero. q fp16
+ * [rows, heads * head_dim] row stride ldq, y fp16 row stride ldy, gate (may be
+ * NULL) fp32 row stride ldg; scores and softmax fp32, the weights rounded to
+ * fp16 as the operand of their product with V. max_tokens: how many tokens the
+ * longest row sees, for the launch's division of long sequences; a row may see
+ * more (slower) or all fewer. Rows in any order of positions.
+ * A row that sees a token whose page id is not below cache->pages, or whose
+ * table entry would lie past ld_table, is NaN; so is one that sees a token of a
+ * block with a NaN scale. Bytes behind a sequence's last seen token may hold
+ * anything. Contract: heads % kv_heads == 0, at most 65,536 heads; scale finite;
+ * ldq % 8 == 0, ldy % 4 == 0, ldg % 4 == 0; q and gate 16-byte, y 8-byte
+ * aligned. Long sequences are divided across workgroups and merged through the
+ * context's forward-kernel workspace (dh_kv8_attention_ws; an eager call of
+ * the same sizes also grows it): the cut depends on the call's sizes only. */
+int dh_kv8_attention(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, uint32_t layer, const dh_kv8_batch* batch,
+                     const uint16_t* q, uint32_t ldq, uint32_t heads, float scale, const float* gate, uint32_t ldg,
+                     uint16_t* y, uint32_t ldy, uint32_t max_tokens);
+/* Grows `stream`'s forward-kernel workspace to what dh_kv8_attention needs for
+ * these sizes (before a capture on that stream, for instance). */
+int dh_kv8_attention_ws(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, uint32_t rows, uint32_t seqs,
+                        uint32_t heads, uint32_t max_tokens);
+
+/* Copies page src[i] to page dst[i] in every layer, i < n (device arrays):
+ * what dh_pages_resize and dh_pages_compact ask for. A pair with an id not
+ * below cache->pages is left out. No dst may be another pair's src or dst. */
+int dh_kv8_copy_pages(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, const uint32_t* src, const uint32_t* dst,
+                      uint32_t n);
+
+/* Which pages which sequence holds: reference counts and tables in host memory,
+ * no device involved. Sequences are numbered 0 .. max_seqs - 1 and start empty;
+ * a new page is always the free one of the lowest id, so equal calls give
+ * equal tables. One dh_pages serves one thread at a time. */
+typedef struct dh_pages dh_pages;
+int dh_pages_create(uint32_t pages, uint32_t max_seqs, dh_pages** out);
+void dh_pages_destroy(dh_pages* p);
+/* Makes sequence s hold `tokens` tokens: frees the pages past them or takes new
+ * ones. Where tokens are added behind a page that is partly full and shared,
+ * the sequence gets a page of its own in its place: copy_src / copy_dst name the
+ * copy to make (dh_kv8_copy_pages) before the tokens are appended, and *copies
+ * is 1 (else 0). If the free pages do not suffice nothing changes and the call
+ * returns DH_ENOMEM. */
+int dh_pages_resize(dh_pages* p, uint32_t seq, uint64_t tokens, uint32_t* copy_src, uint32_t* copy_dst,
+                    uint32_t* copies);
+/* Makes dst (empty before) share the pages of src's first `tokens` tokens. */
+int dh_pages_fork(dh_pages* p, uint32_t src, uint32_t dst, uint64_t tokens);
+/* Moves held pages to the lowest ids: src[i] -> dst[i], i < *moves (arrays of
+ * max entries; as many pages as are held suffice). The tables name the new
+ * pages at once; copy with dh_kv8_copy_pages before the next use. With more
+ * than max moves to make nothing changes and the call returns DH_EINVAL. */
+int dh_pages_compact(dh_pages* p, uint32_t* src, uint32_t* dst, uint32_t max, uint32_t* moves);
+/* A sequence's tokens and pages, and the first min(max, *count) of its page ids. */
+int dh_pages_table(const dh_pages* p, uint32_t seq, uint64_t* tokens, uint32_t* ids, uint32_t max, uint32_t* count);
+/* Free pages, and the sequences that hold page `page`. */
+uint32_t dh_pages_free(const dh_pages* p);
+uint32_t dh_pages_refs(const dh_pages* p, uint32_t page);
+
 #ifdef __cplusplus
 }
 #endif
