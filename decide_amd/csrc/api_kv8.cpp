@@ -197,7 +197,7 @@ int dh_kv8_attention(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, uint3
   if (batch->rows == 0 || batch->seqs == 0) return ok();
   if (!q || !y) return fail(DH_EINVAL, "kv8_attention: null pointer");
   const dh::KvAttnPlan plan = dh::kv8_attention_plan(batch->rows, batch->seqs, heads, cache->kv_heads, cache->head_dim,
-                                                     max_tokens, ctx->cus);
+                                                     batch->ld_table, max_tokens, ctx->cus);
   float* aux = nullptr;
   if (plan.ws_bytes) {
     rc = ensure_aux(ctx, (hipStream_t)stream, plan.ws_bytes, &aux);
@@ -219,8 +219,8 @@ int dh_kv8_attention_ws(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, ui
   if (rc != DH_OK) return rc;
   if (!ctx) return fail(DH_EINVAL, "kv8_attention_ws: null context");
   if (rows == 0 || seqs == 0) return ok();
-  const dh::KvAttnPlan plan =
-      dh::kv8_attention_plan(rows, seqs, heads, cache->kv_heads, cache->head_dim, max_tokens, ctx->cus);
+  const dh::KvAttnPlan plan = dh::kv8_attention_plan(rows, seqs, heads, cache->kv_heads, cache->head_dim,
+                                                     max_tokens / DH_KV8_PAGE + 1, max_tokens, ctx->cus);
   float* aux = nullptr;
   if (plan.ws_bytes) {
     rc = ensure_aux(ctx, (hipStream_t)stream, plan.ws_bytes, &aux);
@@ -251,14 +251,14 @@ int dh_kv8_copy_pages(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, cons
 
 namespace dh_api {
 
-size_t kv8_warm_bytes() { return 65536; }
+size_t kv8_warm_bytes() { return 131072; }
 
 int kv8_warm(dh_ctx* ctx, hipStream_t s, void* mem) {
   // one page of one head of 64 dims at 0 (a second one behind it), everything else zeros: one sequence, one row at
   // position 0, in page 0
   char* const base = (char*)mem;
   const dh_kv8_cache cache{base, 2, 1, 1, 64, DH_KV8_E4M3};
-  static_assert(2 * 8320 <= 32768, "two pages of one head of 64 dims");
+  static_assert(2 * 8320 <= 32768 && 2 * 16 * 66 * 4 + 4 * (dh::kKvMaxSlots + 1) <= 131072 - 49152, "what lies where");
   uint32_t* const u = (uint32_t*)(base + 32768);      // table, row0's 0, qpos, src: zeros
   float* const x = (float*)(base + 36864);
   uint16_t* const y = (uint16_t*)(base + 40960);
@@ -267,8 +267,7 @@ int kv8_warm(dh_ctx* ctx, hipStream_t s, void* mem) {
   int rc = dh_rope(ctx, s, x, 64, 2, y, 64, 0, u, 1, 1, &rope);
   if (rc == DH_OK) rc = dh_kv8_append(ctx, s, &cache, 0, &batch, x, 64, x, 64, 2, &rope);
   if (rc == DH_OK) {
-    dh::KvAttnPlan plan = dh::kv8_attention_plan(1, 1, 1, 1, 64, 1, ctx->cus);
-    plan.np = 2;  // the combine too
+    dh::KvAttnPlan plan{1, 1, 0};  // one run: the combine too
     mark(ctx, kKidKv8Attn);
     mark(ctx, kKidKv8Combine);
     rc = hip_status(dh::launch_kv8_attention(kv_args(&cache, 0, &batch), 64, false, (const _Float16*)x, 64, 1, 1.f,

@@ -38,18 +38,20 @@ hipError_t launch_kv8_append(const KvArgs& a, uint32_t head_dim, bool int8, cons
 hipError_t launch_kv8_copy_pages(uint8_t* pool, uint64_t page_bytes, uint32_t pages, uint32_t layers,
                                  const uint32_t* src, const uint32_t* dst, uint32_t n, hipStream_t s);
 
-// How an attention call is divided: tiles of query rows x heads, and each tile's pages cut every `piece` pages into at
-// most np pieces (the last one takes the rest; np = 1: no cut, no workspace).
+constexpr uint32_t kKvTile = 16;         // (row, head) pairs of a tile
+constexpr uint32_t kKvMaxSlots = 2048;   // tiles that the runs are dealt over (their page counts lie in LDS)
+constexpr uint32_t kKvMinRun = 8;        // pages of a run at least: one for each wave
+
+// How an attention call is divided. runs > 0: the tiles' pages, one after another, in so many equal runs per kv head, a
+// workgroup each, and their states in the workspace: [kv head][run][2] x (O [16][D], (largest score, sum) [16]), then
+// the pages before each tile. runs = 0: a workgroup per tile and kv head, no workspace.
 struct KvAttnPlan {
-  uint32_t tile_rows = 16;  // (row, head) pairs of a tile
-  uint32_t tiles = 0;       // tiles of every kv head, an upper bound
-  uint32_t piece = 1;
-  uint32_t np = 1;
+  uint32_t slots = 0;  // tiles of every kv head, an upper bound
+  uint32_t runs = 0;
   uint64_t ws_bytes = 0;
 };
-constexpr uint32_t kKvMaxPieces = 128;
 KvAttnPlan kv8_attention_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
-                              uint32_t max_tokens, uint32_t cus);
+                              uint32_t ld_table, uint32_t max_tokens, uint32_t cus);
 hipError_t launch_kv8_attention(const KvArgs& a, uint32_t head_dim, bool int8, const _Float16* q, uint32_t ldq,
                                 uint32_t heads, float scale, const float* gate, uint32_t ldg, _Float16* y,
                                 uint32_t ldy, float* ws, const KvAttnPlan& plan, hipStream_t s);

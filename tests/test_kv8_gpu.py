@@ -7,7 +7,7 @@ import pytest
 
 import kv8_reference as ref
 from decide_amd.hip import DeviceArray, Stream, check, rt
-from decide_amd.kernels import Kv8Batch, Kv8Cache, Pages, RopeSpec, rope_freqs
+from decide_amd.kernels import Kernels, Kv8Batch, Kv8Cache, Pages, RopeSpec, rope_freqs
 from gpu_util import full, sync, to_dev, to_host
 
 pytestmark = pytest.mark.gpu
@@ -528,11 +528,12 @@ def test_attention_on_two_streams_at_once(gpu, kernels, stream):
         s.destroy()
 
 
-def test_a_step_replays_from_a_graph(gpu, kernels):
+def test_a_step_replays_from_a_graph(gpu):
     """rope, append, attention of a batch captured once; between replays the positions, rows and tables change and eager work
     runs: every replay is the eager result, byte for byte. A capture that would have to grow the workspace is refused."""
     import ctypes
 
+    kernels = Kernels()  # no workspace from another test
     kv, dim, heads, fmt = 1, 64, 4, "e4m3"
     lens = [5000, 40]
     t = Setup(kv, dim, fmt, [n + 8 for n in lens], [1, 1], layers=1, layer=0, seed=31, behind=0)
@@ -564,11 +565,11 @@ def test_a_step_replays_from_a_graph(gpu, kernels):
         return g, ge
 
     kernels.kv8.attention_ws(s.handle, t.cache, 2, 2, heads, 5008)
-    many = Kv8Batch((u32(np.zeros((1, 4))), 0), 4, (u32([0, 0]), 0), (u32(np.zeros(64)), 0), 1, 64)
-    more = full((64, wide), np.float16, 0)
+    wider = Kv8Cache((t.pool, 0), 1, 1, 1, 256)
+    none = Kv8Batch((u32(np.zeros((1, 100))), 0), 100, (u32([0, 0]), 0), (u32([0]), 0), 1, 1)
+    more = full((1, 256), np.float16, 0)
     with pytest.raises(AssertionError, match="being captured"):
-        capture(lambda: kernels.kv8.attention(s.handle, t.cache, 0, many, (more, 0), wide, heads, 0.125, (more, 0), wide,
-                                              1 << 20))
+        capture(lambda: kernels.kv8.attention(s.handle, wider, 0, none, (more, 0), 256, 1, 0.125, (more, 0), 256, 6400))
     start = to_host(t.pool)
     rows = [np.random.default_rng(i).standard_normal((2, wide + 2 * dim)).astype(np.float32) for i in range(4)]
 
