@@ -77,8 +77,9 @@ dh::KvArgs kv_args(const dh_kv8_cache* c, uint32_t layer, const dh_kv8_batch* b)
 }
 
 int check_heads(const char* op, const dh_kv8_cache* c, uint32_t heads) {
-  if (heads < 1 || heads > 65536 || heads % c->kv_heads != 0)
-    return fail(DH_EINVAL, "%s: heads = %u must be a multiple of the %u kv heads, at most 65536", op, heads, c->kv_heads);
+  if (heads < 1 || heads % c->kv_heads != 0 || heads / c->kv_heads > 1024)
+    return fail(DH_EINVAL, "%s: heads = %u must be a multiple of the %u kv heads, at most 1024 for each", op, heads,
+                c->kv_heads);
   return DH_OK;
 }
 
@@ -267,7 +268,7 @@ int kv8_warm(dh_ctx* ctx, hipStream_t s, void* mem) {
   int rc = dh_rope(ctx, s, x, 64, 2, y, 64, 0, u, 1, 1, &rope);
   if (rc == DH_OK) rc = dh_kv8_append(ctx, s, &cache, 0, &batch, x, 64, x, 64, 2, &rope);
   if (rc == DH_OK) {
-    dh::KvAttnPlan plan{1, 1, 0};  // one run: the combine too
+    dh::KvAttnPlan plan{1, 1, 8, false, 0};  // one run: the combine too
     mark(ctx, kKidKv8Attn);
     mark(ctx, kKidKv8Combine);
     rc = hip_status(dh::launch_kv8_attention(kv_args(&cache, 0, &batch), 64, false, (const _Float16*)x, 64, 1, 1.f,

@@ -40,7 +40,8 @@ hipError_t launch_kv8_copy_pages(uint8_t* pool, uint64_t page_bytes, uint32_t pa
 
 constexpr uint32_t kKvTile = 16;         // (row, head) pairs of a tile
 constexpr uint32_t kKvMaxSlots = 2048;   // tiles that the runs are dealt over (their page counts lie in LDS)
-constexpr uint32_t kKvMinRun = 8;        // pages of a run at least: one for each wave
+constexpr uint32_t kKvWideTile = 128;    // the same for many rows
+constexpr uint32_t kKvWideSlots = 1024;
 
 // How an attention call is divided. runs > 0: the tiles' pages, one after another, in so many equal runs per kv head, a
 // workgroup each, and their states in the workspace: [kv head][run][2] x (O [16][D], (largest score, sum) [16]), then
@@ -48,6 +49,8 @@ constexpr uint32_t kKvMinRun = 8;        // pages of a run at least: one for eac
 struct KvAttnPlan {
   uint32_t slots = 0;  // tiles of every kv head, an upper bound
   uint32_t runs = 0;
+  uint32_t min_run = 1;  // pages of a run at least
+  bool wide = false;
   uint64_t ws_bytes = 0;
 };
 KvAttnPlan kv8_attention_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,

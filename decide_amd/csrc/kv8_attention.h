@@ -1,0 +1,242 @@
+// What the two attention kernels over the 8-bit cache share (kv8_attention.hip, kv8_wide.hip): codes to fp16, tiles of
+// (row, head) pairs, and the runs of pages that workgroups take. Device code only.
+#pragma once
+
+#include "kv8_device.h"
+
+namespace dh {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLazy = 8.0f;  // log2 headroom of the softmax reference point (weights up to 256)
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 8 code bytes (two words) as fp16 numbers, exactly.
+template <bool INT8>
+__device__ __forceinline__ h8 numbers(uint32_t a, uint32_t b) {
+  h2 p[4];
+  if constexpr (INT8) {
+    const h2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+    auto two = [&](uint32_t x, uint32_t sel) {
+      return __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, x, sel)) - bias;
+    };
+    p[0] = two(a, 0x04010400u), p[1] = two(a, 0x04030402u), p[2] = two(b, 0x04010400u), p[3] = two(b, 0x04030402u);
+  } else {
+    p[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false);
+    p[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true);
+    p[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false);
+    p[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true);
+  }
+  h8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[2 * i] = p[i][0], r[2 * i + 1] = p[i][1];
+  return r;
+}
+
+// Combined over the four lanes (n, 0 .. 3) that hold one pair's scores.
+__device__ __forceinline__ float max_groups(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float sum_groups(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+}
+
+__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
+
+// How many tokens row r sees (0 .. 2^32 - 1): its position and those before it; no position wraps to none.
+__device__ __forceinline__ uint32_t seen_by(const KvArgs& a, uint32_t r) { return a.qpos[r] + 1u; }
+
+struct Tile {
+  uint32_t seq;         // sequence
+  uint32_t pairs;       // pairs (rows x group) from the tile's first on, in the sequence
+  uint32_t row, extra;  // the first pair's row, and its head in the group
+};
+
+struct AttnArgs {
+  const _Float16* q;
+  const float* gate;  // or null
+  _Float16* y;
+  float* ws;  // the runs' states (KvAttnPlan)
+  uint32_t ldq, ldg, ldy, heads, group;
+  uint32_t group_inv;  // 2^21 / group, rounded up
+  uint32_t slots;  // tiles are numbered below it
+  uint32_t runs;   // of each kv head; 0: a workgroup per tile
+  uint32_t min_run;
+  float scale;
+};
+
+// Tile `slot` of a kv head: sequences' tiles start at row0 * group / TILE + s, which leaves room for all of them.
+template <uint32_t TILE>
+__device__ __forceinline__ bool tile_of(const KvArgs& a, uint32_t group, uint32_t slot, uint32_t seq, uint32_t begin,
+                                        uint32_t end, Tile& t) {
+  const uint32_t r0 = min(begin, a.rows), r1 = min(end, a.rows);
+  if (r1 <= r0) return false;
+  const uint32_t pairs = (r1 - r0) * group, first = (slot - (uint32_t)((uint64_t)r0 * group / TILE) - seq) * TILE;
+  if (first >= pairs) return false;
+  t = Tile{seq, pairs - first, r0 + first / group, first % group};
+  return true;
+}
+template <uint32_t TILE>
+__device__ __forceinline__ bool find_tile(const KvArgs& a, uint32_t group, uint32_t slot, Tile& t) {
+  const uint32_t s = kv_find_seq(a.row0, a.seqs, a.rows, slot, group, TILE, 1);
+  return s < a.seqs && tile_of<TILE>(a, group, slot, s, a.row0[s], a.row0[s + 1], t);
+}
+// Row and head of the tile's pair k < 128. For x = extra + k < group + 128, x times the rounded 2^21 / group is off by
+// less than x, and x group < 2^21 for groups of at most 1,024: the quotient is exact. (The product stays below 2^32.)
+__device__ __forceinline__ void pair_at(const AttnArgs& t, const Tile& tile, uint32_t kvh, uint32_t k, uint32_t& row,
+                                        uint32_t& head) {
+  const uint32_t x = tile.extra + k, q = x * t.group_inv >> 21;
+  row = tile.row + q;
+  head = kvh * t.group + (x - q * t.group);
+}
+
+// Pages of `seen` tokens. One page past the table is enough to make the row NaN.
+__device__ __forceinline__ uint32_t pages_of(const KvArgs& a, uint32_t seen) {
+  return min(seen / kKvPage + (seen % kKvPage != 0), a.ld_table + 1);
+}
+
+// The runs: run w of `share` pages each, over the tiles' pages one after another.
+__device__ __forceinline__ uint32_t share_of(uint32_t total, const AttnArgs& t) {
+  return max((total + t.runs - 1) / t.runs, t.min_run);
+}
+// Where a run leaves a tile's state: its first tile's at 0, another's that goes on in the next run at 1.
+template <int D, uint32_t TILE>
+__device__ __forceinline__ float* state_of(const AttnArgs& t, uint32_t kvh, uint32_t run, uint32_t which) {
+  return t.ws + ((size_t)(kvh * t.runs + run) * 2 + which) * (TILE * (D + 2));
+}
+// The pages before each tile, left behind the states for the combine.
+template <int D, uint32_t TILE>
+__device__ __forceinline__ uint32_t* starts_of(const KvArgs& a, const AttnArgs& t) {
+  return (uint32_t*)(t.ws + (size_t)a.kv_heads * t.runs * 2 * (TILE * (D + 2)));
+}
+
+// What a workgroup that takes runs keeps in LDS: the pages before each tile, the tile's sequence, the sequences' rows.
+template <uint32_t SLOTS>
+struct Deal {
+  uint32_t before[SLOTS + 1], seq[SLOTS + 1], row0[SLOTS + 1], sums[8];
+};
+
+// Adds up the pages of all tiles, every workgroup for itself (the reads are the same for all and few: each row's position
+// once), and says which pages are this run's.
+template <int D, uint32_t TILE, uint32_t SLOTS, uint32_t THREADS>
+__device__ __forceinline__ void deal_runs(const KvArgs& a, const AttnArgs& t, uint32_t run, Deal<SLOTS>& d, uint32_t& u,
+                                          uint32_t& u1) {
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (uint32_t i = tid; i <= a.seqs; i += THREADS) d.row0[i] = min(a.row0[i], a.rows);
+  __syncthreads();
+#pragma unroll 1
+  for (uint32_t slot = tid; slot < t.slots; slot += THREADS) {
+    uint32_t lo = 0, hi = a.seqs;  // the last sequence that starts at or before the slot
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if ((uint64_t)d.row0[mid] * t.group / TILE + mid <= slot)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    Tile tile;
+    uint32_t most = 0;
+    if ((uint64_t)d.row0[lo] * t.group / TILE + lo <= slot &&
+        tile_of<TILE>(a, t.group, slot, lo, d.row0[lo], d.row0[lo + 1], tile)) {
+      const uint32_t rows = (tile.extra + min(TILE, tile.pairs) - 1) / t.group + 1;
+#pragma unroll 4
+      for (uint32_t r = tile.row; r < tile.row + rows; ++r) most = max(most, seen_by(a, r));
+    }
+    d.seq[slot] = lo;
+    d.before[slot] = pages_of(a, most);
+  }
+  __syncthreads();
+  // running sums: each thread some consecutive tiles, then the lanes, then the waves
+  const uint32_t per = (t.slots + THREADS - 1) / THREADS, at0 = min(tid * per, t.slots), at1 = min(at0 + per, t.slots);
+  uint32_t mine = 0;
+#pragma unroll 1
+  for (uint32_t i = at0; i < at1; ++i) mine += d.before[i];
+  uint32_t sum = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t v = (uint32_t)__shfl_up((int)sum, o, 64);
+    if (lane >= (uint32_t)o) sum += v;
+  }
+  if (lane == 63) d.sums[wave] = sum;
+  __syncthreads();
+  uint32_t at = sum - mine, total = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < THREADS / 64; ++w) {
+    at += w < wave ? d.sums[w] : 0;
+    total += d.sums[w];
+  }
+#pragma unroll 1
+  for (uint32_t i = at0; i < at1; ++i) {
+    const uint32_t n = d.before[i];
+    d.before[i] = at;
+    at += n;
+  }
+  if (tid == 0) d.before[t.slots] = total;
+  __syncthreads();
+  total = (uint32_t)__builtin_amdgcn_readfirstlane((int)total);
+  if (blockIdx.x == 0) {
+    uint32_t* const out = starts_of<D, TILE>(a, t);
+#pragma unroll 1
+    for (uint32_t i = tid; i <= t.slots; i += THREADS) out[i] = d.before[i];
+  }
+  const uint32_t share = share_of(total, t);
+  u = (uint32_t)min((uint64_t)run * share, (uint64_t)total);
+  u1 = min(u + share, total);
+}
+
+// The tile that holds page u of a kv head: the last that starts at or before it (empty ones start where the next does).
+template <uint32_t SLOTS>
+__device__ __forceinline__ uint32_t tile_at(const Deal<SLOTS>& d, uint32_t slots, uint32_t u) {
+  uint32_t lo = 0, hi = slots;
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (d.before[mid] <= u)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// Four outputs of row r: O times `factor`, times the gate's sigmoid.
+template <bool GATE>
+__device__ __forceinline__ void store_out(const AttnArgs& t, uint32_t r, uint32_t col, const f4& acc, float factor) {
+  f4 v = acc * factor;
+  if constexpr (GATE) {
+    const f4 gt = *(const f4*)(t.gate + (size_t)r * t.ldg + col);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= sigmoid(gt[e]);
+  }
+  *(h4*)(t.y + (size_t)r * t.ldy + col) = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+}
+
+__device__ __forceinline__ void store_out(const AttnArgs& t, uint32_t r, uint32_t col, const f4& acc, float factor) {
+  if (t.gate)
+    store_out<true>(t, r, col, acc, factor);
+  else
+    store_out<false>(t, r, col, acc, factor);
+}
+__device__ __forceinline__ float over_sum(float l) { return l == 0.f ? 0.f : 1.0f / l; }  // a row that sees nothing is 0
+
+// weight of a state whose reference point is m among those whose largest is top; none where it met no score
+__device__ __forceinline__ float state_weight(float m, float top) {
+  return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+}
+
+// kv8_wide.hip: the kernel for many rows, over t.runs runs or t.slots tiles
+hipError_t launch_kv8_wide(const KvArgs& a, const AttnArgs& t, uint32_t head_dim, bool int8, hipStream_t s);
+
+}  // namespace dh

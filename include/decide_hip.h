@@ -632,7 +632,7 @@ int dh_kv8_append(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, uint32_t
  * A row that sees a token whose page id is not below cache->pages, or whose
  * table entry would lie past ld_table, is NaN; so is one that sees a token of a
  * block with a NaN scale. Bytes behind a sequence's last seen token may hold
- * anything. Contract: heads % kv_heads == 0, at most 65,536 heads; scale finite;
+ * anything. Contract: heads % kv_heads == 0, at most 1,024 heads a kv head; scale finite;
  * ldq % 8 == 0, ldy % 4 == 0, ldg % 4 == 0; q and gate 16-byte, y 8-byte
  * aligned. Long sequences are divided across workgroups and merged through the
  * context's forward-kernel workspace (dh_kv8_attention_ws; an eager call of

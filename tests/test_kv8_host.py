@@ -102,7 +102,7 @@ def test_append_refusals(kw, msg):
 
 @pytest.mark.parametrize("kw,msg", [
     (dict(layer=7), "layer 7 of 2"), (dict(heads=0), "multiple of the 4 kv heads"), (dict(heads=18), "multiple of"),
-    (dict(heads=65540), "at most 65536"), (dict(scale=math.nan), "scale"), (dict(q=8), "q must be"),
+    (dict(heads=4100), "at most 1024"), (dict(scale=math.nan), "scale"), (dict(q=8), "q must be"),
     (dict(ldq=4092), "ldq"), (dict(ldq=4100), "ldq"), (dict(y=4), "y must be"), (dict(ldy=4090), "ldy"),
     (dict(gate=8), "gate must be"), (dict(ldg=4000), "ldg"), (dict(batch=dict(rows=1 << 29)), "one launch"),
 ])
