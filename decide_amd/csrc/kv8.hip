@@ -19,27 +19,26 @@ namespace {
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef uint16_t us4 __attribute__((ext_vector_type(4)));
 
-// N (1, 2 or 4) elements of dtype T as floats
+// N (1, 2 or 4) elements of dtype T (float, Half, Bf16), as they lie in memory and as floats. Loads come before the
+// branches that use them, so that a wave's are all in flight at once.
 struct Half {};
 struct Bf16 {};
-
 template <typename T, int N>
-__device__ __forceinline__ void load_n(const void* base, size_t at, float* out) {
+struct Raw {
   typedef std::conditional_t<std::is_same_v<T, float>, float, uint16_t> E;
   struct alignas(N * sizeof(E)) Pack {
     E e[N];
-  };
-  const Pack x = *(const Pack*)((const E*)base + at);
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
+  } v;
+  __device__ __forceinline__ void load(const void* base, size_t at) { v = *(const Pack*)((const E*)base + at); }
+  __device__ __forceinline__ float operator[](int i) const {
     if constexpr (std::is_same_v<T, float>)
-      out[i] = x.e[i];
+      return v.e[i];
     else if constexpr (std::is_same_v<T, Half>)
-      out[i] = (float)__builtin_bit_cast(_Float16, x.e[i]);
+      return (float)__builtin_bit_cast(_Float16, v.e[i]);
     else
-      out[i] = __uint_as_float((uint32_t)x.e[i] << 16);
+      return __uint_as_float((uint32_t)v.e[i] << 16);
   }
-}
+};
 
 __device__ __forceinline__ uint16_t to_bf16(float x) {
   const uint32_t u = __float_as_uint(x);
@@ -64,78 +63,184 @@ __device__ __forceinline__ double half_turns(double pos, float f) {
   return t - 2.0 * rint(0.5 * t) + low;
 }
 
-// R(1) / sqrt(mean of squares + eps) over a head held 4 elements a lane by W lanes
+// The value of the lane `ror` further on within its row of 16.
+template <int ROR>
+__device__ __forceinline__ uint32_t row_rotate(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + ROR, 0xf, 0xf, false);
+}
+template <int ROR, typename R>
+__device__ __forceinline__ R rotated(R x) {
+  if constexpr (sizeof(R) == 4) {
+    return __builtin_bit_cast(R, row_rotate<ROR>(__builtin_bit_cast(uint32_t, x)));
+  } else {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    return __builtin_bit_cast(R, (uint64_t)row_rotate<ROR>((uint32_t)u) | (uint64_t)row_rotate<ROR>((uint32_t)(u >> 32)) << 32);
+  }
+}
+// x of the lanes that differ in bit 4 (H = 16) or 5 (32), combined by f
+template <int H, typename R, typename F>
+__device__ __forceinline__ R across(R x, F f) {
+  auto swap = [](uint32_t v) {
+    if constexpr (H == 16)
+      return __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    else
+      return __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  };
+  if constexpr (sizeof(R) == 4) {
+    const auto p = swap(__builtin_bit_cast(uint32_t, x));
+    return f(__builtin_bit_cast(R, (uint32_t)p[0]), __builtin_bit_cast(R, (uint32_t)p[1]));
+  } else {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const auto lo = swap((uint32_t)u), hi = swap((uint32_t)(u >> 32));
+    return f(__builtin_bit_cast(R, (uint64_t)lo[0] | (uint64_t)hi[0] << 32),
+             __builtin_bit_cast(R, (uint64_t)lo[1] | (uint64_t)hi[1] << 32));
+  }
+}
+// f over the W (16, 32 or 64) lanes of a group, in every lane: register moves, no LDS
+template <int W, typename R, typename F>
+__device__ __forceinline__ R reduce(R x, F f) {
+  x = f(x, rotated<8>(x));
+  x = f(x, rotated<4>(x));
+  x = f(x, rotated<2>(x));
+  x = f(x, rotated<1>(x));
+  if constexpr (W >= 32) x = across<16>(x, f);
+  if constexpr (W >= 64) x = across<32>(x, f);
+  return x;
+}
+
+// How a lane's elements d .. d + 3 of a head are normed and turned: their weights and where their pairs are. `quick`:
+// all four turn or none does, and their pairs lie in one other lane or in this one.
+template <typename R>
+struct Turn {
+  R w[4], wo[4];     // weights of the four and of what they pair with (1 without a norm)
+  uint32_t d, pair;  // pair: the first's number
+  uint32_t partner;  // the lane that holds what they pair with
+  bool quick, turns, first;
+  __device__ __forceinline__ void init(const RopeArgs& p, uint32_t lane, uint32_t width, R add) {
+    d = 4 * lane;
+    quick = p.interleaved ? p.rot % 4 == 0 : p.rot % 8 == 0;
+    turns = d < p.rot;
+    first = d < p.rot / 2;
+    pair = p.interleaved ? d / 2 : first ? d : d - p.rot / 2;
+    partner = p.interleaved || !turns ? lane : first ? lane + p.rot / 8 : lane - p.rot / 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = p.norm_w && d < width ? (R)p.norm_w[d + i] + add : (R)1;
+      wo[i] = p.norm_w && d < width ? (R)p.norm_w[4 * partner % width + i] + add : (R)1;
+    }
+  }
+};
+
+// Normed and turned: x the lane's own values, at base[at + d] in memory, inv the head's norm factor, cs (cos, sin) of
+// each pair. Every lane of the head's group calls it. The products and sums are spelled out, so that the same row gets
+// the same bits wherever it stands.
+template <typename T, int W, typename R>
+__device__ __forceinline__ void turn4(const float* x, const void* base, size_t at, const RopeArgs& p, const Turn<R>& t,
+                                      R inv, R (*cs)[2], R* y) {
+  auto low = [](R a, R c, R b, R s) { return fma(a, c, -(b * s)); };
+  auto high = [](R a, R c, R b, R s) { return fma(a, c, b * s); };
+  R z[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = z[i] = (R)x[i] * (inv * t.w[i]);
+  if (t.quick) {
+    if (p.interleaved) {
+      if (t.turns) {
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const R c = cs[t.pair + i / 2][0], s = cs[t.pair + i / 2][1];
+          y[i] = low(z[i], c, z[i + 1], s);
+          y[i + 1] = high(z[i + 1], c, z[i], s);
+        }
+      }
+    } else {
+      R o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = (R)__shfl(x[i], (int)t.partner, W) * (inv * t.wo[i]);
+      if (t.turns) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const R c = cs[t.pair + i][0], s = cs[t.pair + i][1];
+          y[i] = t.first ? low(z[i], c, o[i], s) : high(z[i], c, o[i], s);
+        }
+      }
+    }
+    return;
+  }
+  const uint32_t half = p.rot / 2;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t e = t.d + i;
+    if (e >= p.rot) continue;
+    const uint32_t with = p.interleaved ? e ^ 1 : e < half ? e + half : e - half;
+    const bool first = p.interleaved ? !(e & 1) : e < half;
+    const uint32_t pair = p.interleaved ? e / 2 : first ? e : e - half;
+    Raw<T, 1> r;
+    r.load(base, at + with);  // in the lines that this wave has just read
+    const R o = (R)r[0] * (inv * (p.norm_w ? (R)p.norm_w[with] + (R)(p.add_one ? 1 : 0) : (R)1));
+    const R c = cs[pair][0], s = cs[pair][1];
+    y[i] = first ? low(z[i], c, o, s) : high(z[i], c, o, s);
+  }
+}
+
+// 1 / sqrt(mean of squares + eps) over a head held 4 elements a lane by W lanes
 template <int W, typename R>
 __device__ __forceinline__ R norm_factor(const float* x, uint32_t head_dim, float eps) {
   R ss = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) ss += (R)x[i] * (R)x[i];
-#pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, W);
+  for (int i = 0; i < 4; ++i) ss = fma((R)x[i], (R)x[i], ss);
+  ss = reduce<W>(ss, [](R a, R b) { return a + b; });
   if constexpr (std::is_same_v<R, double>)
-    return 1.0 / sqrt(ss / (double)head_dim + (double)eps);
+    return rsqrt(ss / (double)head_dim + (double)eps);
   else
     return 1.0f / sqrtf(ss / (float)head_dim + eps);
-}
-
-// The lane's elements d .. d + 3 of a head, normed and turned. x: the lane's own values; base[at ..]: the head (the
-// values that x pairs with are read there again: they lie in the lines that this wave has just read); cs: (cos, sin) of
-// each pair.
-template <typename T, typename R>
-__device__ __forceinline__ void rope4(const float* x, const void* base, size_t at, uint32_t d, const RopeArgs& p, R inv,
-                                      R (*cs)[2], R* y) {
-  const uint32_t half = p.rot / 2;
-  auto weight = [&](uint32_t e) { return p.norm_w ? inv * ((R)p.norm_w[e] + (R)(p.add_one ? 1 : 0)) : (R)1; };
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t e = d + i;
-    y[i] = (R)x[i] * weight(e);
-    if (e < p.rot) {
-      R other;
-      uint32_t pair;
-      bool first;
-      if (p.interleaved) {
-        pair = e / 2;
-        first = !(e & 1);
-        other = (R)x[i ^ 1] * weight(e ^ 1);
-      } else {
-        first = e < half;
-        pair = first ? e : e - half;
-        const uint32_t o = first ? e + half : e - half;
-        float ox;
-        load_n<T, 1>(base, at + o, &ox);
-        other = (R)ox * weight(o);
-      }
-      const R c = cs[pair][0], s = cs[pair][1];
-      y[i] = first ? y[i] * c - other * s : y[i] * c + other * s;
-    }
-  }
 }
 
 // ---- rope ----------------------------------------------------------------------------------------------------------
 template <typename TX, typename TY, int W>
 __global__ __launch_bounds__(256) void rope_kernel(const void* x, uint32_t ldx, void* y, uint32_t ldy,
                                                    const uint32_t* __restrict__ pos, uint32_t heads, RopeArgs p) {
+  constexpr uint32_t kAtOnce = 4;  // heads that a group of lanes has in flight
   __shared__ float cs[128][2];
-  const uint32_t r = blockIdx.x, tid = threadIdx.x;
+  const uint32_t r = blockIdx.x, tid = threadIdx.x, lane = tid % W;
+  const bool mine = 4 * lane < p.head_dim;
+  const uint32_t d = mine ? 4 * lane : 0;
+  Raw<TX, 4> raw[kAtOnce];
+  auto load = [&](uint32_t h0) {
+#pragma unroll
+    for (uint32_t j = 0; j < kAtOnce; ++j) {
+      const uint32_t h = min(h0 + j * (256 / W), heads - 1);
+      raw[j].load(x, (size_t)r * ldx + (size_t)h * p.head_dim + d);
+    }
+  };
+  load(tid / W);
+  Turn<float> turn;
+  turn.init(p, lane, p.head_dim, p.add_one ? 1.f : 0.f);
   if (tid < p.rot / 2) {
-    const double t = half_turns(pos[r], p.inv_freq[tid]);
+    const double t = half_turns((double)pos[r], p.inv_freq[tid]);
     float s, c;
     sincospif((float)t, &s, &c);
     cs[tid][0] = c * p.amp;
     cs[tid][1] = s * p.amp;
   }
   __syncthreads();
-  const uint32_t d = 4 * (tid % W);
-  for (uint32_t h = tid / W; h < heads; h += 256 / W) {
-    const size_t at = (size_t)r * ldx + (size_t)h * p.head_dim;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (d < p.head_dim) load_n<TX, 4>(x, at + d, v);
-    const float inv = p.norm_w ? norm_factor<W, float>(v, p.head_dim, p.eps) : 1.0f;
-    float o[4];
-    if (d < p.head_dim) rope4<TX, float>(v, x, at, d, p, inv, cs, o);
+  for (uint32_t h0 = tid / W; h0 < heads; h0 += kAtOnce * (256 / W)) {
+    if (h0 != tid / W) load(h0);
+    float o[kAtOnce][4];
+#pragma unroll
+    for (uint32_t j = 0; j < kAtOnce; ++j) {
+      const uint32_t h = min(h0 + j * (256 / W), heads - 1);
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = mine ? raw[j][i] : 0.f;
+      const float inv = p.norm_w ? norm_factor<W, float>(v, p.head_dim, p.eps) : 1.0f;
+      turn4<TX, W, float>(v, x, (size_t)r * ldx + (size_t)h * p.head_dim, p, turn, inv, cs, o[j]);
+    }
     __builtin_amdgcn_wave_barrier();  // y may be x: every lane has read its pairs before one stores
-    if (d < p.head_dim) store4<TY>(y, (size_t)r * ldy + (size_t)h * p.head_dim + d, o);
+#pragma unroll
+    for (uint32_t j = 0; j < kAtOnce; ++j) {
+      const uint32_t h = h0 + j * (256 / W);
+      if (mine && h < heads) store4<TY>(y, (size_t)r * ldy + (size_t)h * p.head_dim + d, o[j]);
+    }
   }
 }
 
@@ -156,10 +261,12 @@ __device__ __forceinline__ float block_scale(float amax) {
   }
 }
 
-// x / scale; a scale that is a power of two has an exact reciprocal.
+// x / scale, correctly rounded, with inv = 1 / scale correctly rounded: a power of two has an exact reciprocal; otherwise
+// the product's remainder, exact in a fused multiply-add, corrects it (Markstein's division).
 template <bool INT8>
 __device__ __forceinline__ float scaled(float x, float scale, float inv) {
-  return INT8 ? x / scale : x * inv;
+  const float q = x * inv;
+  return INT8 ? fmaf(fmaf(-q, scale, x), inv, q) : q;
 }
 
 // Four values, divided by their scale, as code bytes (round to nearest even; e4m3 to e4m3 in the hardware's conversion).
@@ -193,12 +300,6 @@ __device__ __forceinline__ uint32_t recode4(uint32_t u, float ratio) {
   return code4<INT8>(v[0] * ratio, v[1] * ratio, v[2] * ratio, v[3] * ratio);
 }
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
-  return x;
-}
-
 // Largest magnitude of a wave's values and whether all are finite, then the block's scale: `keep` tokens stay with theirs.
 template <bool INT8, int N>
 __device__ __forceinline__ float new_scale(const float* x, bool keep, float before) {
@@ -209,7 +310,7 @@ __device__ __forceinline__ float new_scale(const float* x, bool keep, float befo
     amax = fmaxf(amax, fabsf(x[i]));
     finite = finite && fabsf(x[i]) < INFINITY;
   }
-  const float s = block_scale<INT8>(wave_max(amax));
+  const float s = block_scale<INT8>(reduce<64>(amax, [](float a, float b) { return fmaxf(a, b); }));
   if (!__all(finite) || (keep && before != before)) return NAN;
   return keep ? fmaxf(s, before) : s;
 }
@@ -224,10 +325,9 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(KvArgs a, const void* _
   __shared__ double cs[4][4][128][2];
   const uint32_t head = blockIdx.y % a.kv_heads;
   const bool is_v = blockIdx.y >= a.kv_heads;
-  const uint32_t s = kv_find_seq(a.row0, a.seqs, a.rows, blockIdx.x, 1, kKvPage, 2);
-  if (s >= a.seqs) return;
-  const uint32_t r0 = min(a.row0[s], a.rows), r1 = min(a.row0[s + 1], a.rows);
-  if (r1 <= r0) return;
+  uint32_t r0, r1;
+  const uint32_t s = kv_find_seq(a.row0, a.seqs, a.rows, blockIdx.x, 1, kKvPage, 2, r0, r1);
+  if (s >= a.seqs || r1 <= r0) return;
   const uint64_t p0 = a.qpos[r0], p1 = p0 + (r1 - r0);  // the tokens p0 .. p1 - 1 are new
   const uint64_t page = p0 / kKvPage + (blockIdx.x - (r0 / kKvPage + 2 * s));
   const uint32_t lane = threadIdx.x & 63, block = threadIdx.x >> 6;
@@ -241,50 +341,91 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(KvArgs a, const void* _
   const uint32_t end = p1 < t0 + kKvBlock ? (uint32_t)(p1 - t0) : kKvBlock;  // its new tokens are kept .. end - 1
   const float before = kept ? *scale : 0.f;
   const size_t row = r0 + (size_t)(t0 - p0);  // the row of the block's token 0 (wraps below zero before row r0)
-  constexpr uint32_t kZero = INT8 ? 0x80808080u : 0u;
 
   if (is_v) {
     constexpr int C = D / 64;  // dims of a lane, all 16 tokens
     const uint32_t d = lane * C;
+    Raw<T, C> raw[kKvBlock];
+#pragma unroll
+    for (uint32_t t = 0; t < kKvBlock; ++t)  // a row of the call in place of those that are none of it
+      raw[t].load(v, (row + min(max(t, kept), end - 1)) * ldv + head * D + d);
+    uint8_t* const at = rec + kv_v_at<D>(head, a.kv_heads) + (size_t)d * kKvPage + block * kKvBlock;
+    u4 old[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) old[c] = kept ? *(const u4*)(at + c * kKvPage) : u4{0, 0, 0, 0};
     float x[kKvBlock][C];
 #pragma unroll
-    for (uint32_t t = 0; t < kKvBlock; ++t) {
+    for (uint32_t t = 0; t < kKvBlock; ++t)
 #pragma unroll
-      for (int c = 0; c < C; ++c) x[t][c] = 0.f;
-      if (t >= kept && t < end) load_n<T, C>(v, (row + t) * ldv + head * D + d, x[t]);
-    }
+      for (int c = 0; c < C; ++c) x[t][c] = t >= kept && t < end ? raw[t][c] : 0.f;
     const float sc = new_scale<INT8, kKvBlock * C>(&x[0][0], kept != 0, before);
-    const float ratio = before / sc, inv = 1.0f / sc;
+    const float inv = 1.0f / sc;
     if (lane == 0) *scale = sc;
-    uint8_t* const at = rec + kv_v_at<D>(head, a.kv_heads) + (size_t)d * kKvPage + block * kKvBlock;
+    if (kept) {
+      if (sc > before) {
+        const float ratio = before / sc;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) old[c][w] = recode4<INT8>(old[c][w], ratio);
+      }
+    }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      u4 out, old = u4{0, 0, 0, 0};
-      if (kept) old = *(const u4*)(at + c * kKvPage);
+      u4 out;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         float q[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) q[i] = sc == sc ? scaled<INT8>(x[4 * w + i][c], sc, inv) : 0.f;
-        const uint32_t fresh = code4<INT8>(q[0], q[1], q[2], q[3]);
-        const uint32_t stay = sc == before || sc != sc ? old[w] : recode4<INT8>(old[w], ratio);
-        uint32_t m = 0;  // bytes of tokens that stay
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m |= 4 * w + i < (int)kept ? 255u << 8 * i : 0u;
-        out[w] = (stay & m) | (fresh & ~m);
+        const int stay = (int)kept - 4 * w;  // bytes of tokens that stay
+        const uint32_t m = stay >= 4 ? ~0u : stay <= 0 ? 0u : (1u << 8 * stay) - 1u;
+        out[w] = (old[c][w] & m) | (code4<INT8>(q[0], q[1], q[2], q[3]) & ~m);
       }
       *(u4*)(at + c * kKvPage) = out;
     }
     return;
   }
 
+  // K: pass n holds token n TP + lane / W, 4 dims a lane
   const uint32_t d = 4 * (lane % W);
-  float x[P][4];
+  auto token = [&](int n) { return n * TP + lane / W; };
+  auto source = [&](int n) { return (row + min(max(token(n), kept), end - 1)) * ldk + head * D; };
+  Raw<T, 4> raw[P];
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {  // four tokens share a table of angles
-    if (rope.inv_freq && 4u * g < end && 4u * g + 4 > kept) {
-      for (uint32_t i = lane; i < 2 * rope.rot; i += 64) {
-        const uint32_t pair = i % (rope.rot / 2), t = i / (rope.rot / 2);
+  for (int n = 0; n < P; ++n) raw[n].load(k, source(n) + d);
+  // the block as it was, 16 bytes a lane
+  constexpr int B = D / 64;
+  uint8_t* const base = rec + kv_k_at<D>(head) + (size_t)block * kKvBlock * D;
+  u4 old[B];
+#pragma unroll
+  for (int j = 0; j < B; ++j) old[j] = kept ? *(const u4*)(base + j * 1024 + lane * 16) : u4{0, 0, 0, 0};
+  float x[P][4];
+  if (rope.inv_freq) {
+    Turn<double> turn;
+    turn.init(rope, lane % W, D, rope.add_one ? 1.0 : 0.0);
+    auto pass = [&](int n) {
+      float own[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) own[i] = raw[n][i];
+      const double inv = rope.norm_w ? norm_factor<W, double>(own, D, rope.eps) : 1.0;
+      double y[4];
+      turn4<T, W, double>(own, k, source(n), rope, turn, inv, cs[block][token(n) % 4], y);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[n][i] = (float)y[i];
+    };
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {  // four tokens share a table of angles
+#pragma unroll
+      for (int j = 0; j < P / 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[g * (P / 4) + j][i] = 0.f;
+      if (4u * g >= end || 4u * g + 4 <= kept) continue;
+      __builtin_amdgcn_wave_barrier();
+      const uint32_t pairs = rope.rot / 2;
+      for (uint32_t i = lane; i < 4 * pairs; i += 64) {
+        const uint32_t pair = i % pairs, t = i / pairs;
+        if (4 * g + t < kept || 4 * g + t >= end) continue;
         double sn, c;
         sincospi(half_turns((double)(t0 + 4 * g + t), rope.inv_freq[pair]), &sn, &c);
         cs[block][t][pair][0] = c * (double)rope.amp;
@@ -292,44 +433,50 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(KvArgs a, const void* _
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // this wave's own reads follow
       __builtin_amdgcn_wave_barrier();
-    }
+      if (4u * g >= kept && 4u * g + 4 <= end) {
 #pragma unroll
-    for (int j = 0; j < P / 4; ++j) {
-      const int n = g * (P / 4) + j;
-      const uint32_t t = n * TP + lane / W;
+        for (int j = 0; j < P / 4; ++j) pass(g * (P / 4) + j);
+      } else {  // a new token or two: only the passes that hold them
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[n][i] = 0.f;
-      const bool fresh = t >= kept && t < end;
-      const size_t at = (row + t) * ldk + head * D;
-      if (fresh) load_n<T, 4>(k, at + d, x[n]);
-      if (rope.inv_freq) {
-        const double inv = rope.norm_w ? norm_factor<W, double>(x[n], D, rope.eps) : 1.0;
-        if (fresh) {
-          double y[4];
-          rope4<T, double>(x[n], k, at, d, rope, inv, cs[block][t % 4], y);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[n][i] = (float)y[i];
+        for (int j = 0; j < P / 4; ++j) {
+          const uint32_t n = g * (P / 4) + j;
+          if (n * TP < end && n * TP + TP > kept) pass(n);
         }
       }
     }
-    __builtin_amdgcn_wave_barrier();
+  } else {
+#pragma unroll
+    for (int n = 0; n < P; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[n][i] = raw[n][i];
   }
-  const float sc = new_scale<INT8, P * 4>(&x[0][0], kept != 0, before);
-  const float ratio = before / sc, inv = 1.0f / sc;
-  if (lane == 0) *scale = sc;
-  uint8_t* const base = rec + kv_k_at<D>(head) + (size_t)block * kKvBlock * D + d;
 #pragma unroll
   for (int n = 0; n < P; ++n) {
-    const uint32_t t = n * TP + lane / W;
-    uint32_t* const at = (uint32_t*)(base + t * D);
-    if (t < kept) {
-      if (sc > before) *at = recode4<INT8>(*at, ratio);
-    } else if (t < end && sc == sc) {
-      *at = code4<INT8>(scaled<INT8>(x[n][0], sc, inv), scaled<INT8>(x[n][1], sc, inv), scaled<INT8>(x[n][2], sc, inv),
-                        scaled<INT8>(x[n][3], sc, inv));
-    } else {
-      *at = kZero;
+    const uint32_t t = token(n);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[n][i] = t >= kept && t < end ? x[n][i] : 0.f;
+  }
+  const float sc = new_scale<INT8, P * 4>(&x[0][0], kept != 0, before);
+  const float inv = 1.0f / sc;
+  if (lane == 0) *scale = sc;
+  if (kept && sc > before) {
+    const float ratio = before / sc;
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      if ((j * 1024 + lane * 16) / D >= kept) continue;
+      u4 now;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) now[w] = recode4<INT8>(old[j][w], ratio);
+      *(u4*)(base + j * 1024 + lane * 16) = now;
     }
+  }
+#pragma unroll
+  for (int n = 0; n < P; ++n) {
+    const uint32_t t = token(n);
+    float q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = sc == sc ? scaled<INT8>(x[n][i], sc, inv) : 0.f;
+    if (t >= kept) *(uint32_t*)(base + t * D + d) = code4<INT8>(q[0], q[1], q[2], q[3]);
   }
 }
 

@@ -91,8 +91,9 @@ __device__ __forceinline__ bool tile_of(const KvArgs& a, uint32_t group, uint32_
 }
 template <uint32_t TILE>
 __device__ __forceinline__ bool find_tile(const KvArgs& a, uint32_t group, uint32_t slot, Tile& t) {
-  const uint32_t s = kv_find_seq(a.row0, a.seqs, a.rows, slot, group, TILE, 1);
-  return s < a.seqs && tile_of<TILE>(a, group, slot, s, a.row0[s], a.row0[s + 1], t);
+  uint32_t begin, end;
+  const uint32_t s = kv_find_seq(a.row0, a.seqs, a.rows, slot, group, TILE, 1, begin, end);
+  return s < a.seqs && tile_of<TILE>(a, group, slot, s, begin, end, t);
 }
 // Row and head of the tile's pair k < 128. For x = extra + k < group + 128, x times the rounded 2^21 / group is off by
 // less than x, and x group < 2^21 for groups of at most 1,024: the quotient is exact. (The product stays below 2^32.)

@@ -286,7 +286,7 @@ KvAttnPlan kv8_attention_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint
   const uint64_t pages = std::min<uint64_t>(((uint64_t)max_tokens + kKvPage - 1) / kKvPage, ld_table);
   if (pages <= (p.wide ? 4 : 16) || slots > (p.wide ? kKvWideSlots : kKvMaxSlots) || slots * (ld_table + 1ull) > UINT32_MAX) return p;
   static const char* fr = getenv("KV8_RUNS");
-  const int mul = fr ? atoi(fr) : p.wide ? 2 : 1;
+  const int mul = fr ? atoi(fr) : p.wide && slots * kv_heads >= cus ? 0 : 1;
   if (mul == 0) return p;
   p.runs = std::max<uint32_t>(1, mul * cus / kv_heads);
   static const char* fm = getenv("KV8_MIN");

@@ -1,13 +1,17 @@
 // Attention over the 8-bit paged cache where many rows share their tokens (prompts, long follow-ups), for gfx950 MFMA.
 //
-// kv8_attention_wide_kernel, tiles of 128 (row, head) pairs: four waves of 32 pairs, on v_mfma_f32_32x32x16_f16.
-//   * The tile's pages go into LDS as they are, by DMA, two buffers; every wave reads all of a page's codes from there
-//     and turns them into fp16 in registers. 32 pairs a wave make 64 products of 32 clocks of a page against 64 reads
-//     of 16 bytes a lane (1,024 clocks a CU for two workgroups' ... ) and 256 conversions.
-//   * The same deal of tokens as in kv8_attention_kernel, for two lane groups: over 32 keys (T = 0, 1) lane (r, f), r = lane % 32, f =
-//     lane / 32, gets the 16 scores of pair r and block 2 T + f, which are P^T V's operand as they are.
+// kv8_attention_wide_kernel, tiles of 128 (row, head) pairs: eight waves, four groups of 32 pairs x the two halves of a
+// page's blocks, on v_mfma_f32_32x32x16_f16.
+//   * Pages go into LDS as they are, by DMA, two at a time into one of two buffers, one barrier per two pages; a wave
+//     reads the codes of its half from there and turns them into fp16 in registers, 128 conversions and 32 products of
+//     32 clocks a page.
+//   * The same deal of tokens as in kv8_attention_kernel, for two lane groups: lane (r, f), r = lane % 32, f = lane / 32,
+//     of half T gets the 16 scores of pair r and block 2 T + f, which are P^T V's operand as they are.
 //   * 16-byte chunk x of K's token t lies at chunk x ^ key(t), of V's dim d at x ^ (d / 2 % 4), so that eight lanes
 //     that read at once read 128 different bytes' banks.
+//   * Two waves of a SIMD share its issue port: alone, a wave issues an instruction of the vector unit every 6 to 7 clocks,
+//     two together one every 4. With four waves a workgroup, both halves a wave, 37 pages took 96 us against XX.
+//   * The two halves meet once, at a tile's end, through LDS: each takes half of the dims.
 #include "kv8_attention.h"
 
 namespace dh {
@@ -38,31 +42,36 @@ typedef const __attribute__((address_space(4))) uint32_t* scalar_words;
 }  // namespace
 
 template <int D, bool INT8, bool RUNS>
-__global__ __launch_bounds__(256, 2) void kv8_attention_wide_kernel(KvArgs a, AttnArgs t) {
-  constexpr int C = D / 32;  // pairs of 16-byte chunks of a key
+__global__ __launch_bounds__(512) void kv8_attention_wide_kernel(KvArgs a, AttnArgs t) {
+  constexpr int C = D / 32;   // pairs of 16-byte chunks of a key
   constexpr int DT = D / 32;  // 32-dim tiles of O
-  constexpr uint32_t kBytes = kKvPage * D;
-  __shared__ __attribute__((aligned(1024))) char lds[4 * kBytes];  // two pages of K, two of V
+  constexpr uint32_t kBytes = kKvPage * D;  // of a page's K, or V
+  constexpr uint32_t kPieces = kBytes / 4096;
+  constexpr int kAhead = D == 256 ? 2 : 3;  // LDS reads ahead of their products (registers allow no third)
+  // four pages (K, V); at a tile's end the halves' O: [wave][DT / 2 x 4 pieces of 4 dims][64 lanes]
+  __shared__ __attribute__((aligned(1024))) char lds[8 * kBytes];
+  static_assert(8 * (DT / 2 * 4) * 64 * 16 <= sizeof(lds), "the halves' exchange fits the pages");
+  __shared__ __attribute__((aligned(1024))) float scales[4][256];  // of the pages: K's 4, V's 4 (a DMA's room)
+  __shared__ f4 meet[8 * 32];                                      // largest score, sum, V scale of each wave's pairs
   __shared__ Deal<RUNS ? kKvWideSlots : 0> deal;
-  __shared__ __attribute__((aligned(1024))) float scales[2][256];  // of the two pages: K's 4, V's 4 (a DMA's room)
-  __shared__ uint32_t seen_most[4];
+  __shared__ uint32_t seen_most[8];
   const uint32_t kvh = blockIdx.x % a.kv_heads, run = blockIdx.x / a.kv_heads;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = wave & 3, T = wave >> 2;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   const uint32_t scales0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)scales;
   uint32_t u = 0, u1 = 1;
-  if constexpr (RUNS) deal_runs<D, kKvWideTile, kKvWideSlots, 256>(a, t, run, deal, u, u1);
+  if constexpr (RUNS) deal_runs<D, kKvWideTile, kKvWideSlots, 512>(a, t, run, deal, u, u1);
   const uint32_t first_u = u;
   const float c = fabsf(t.scale) * kLog2e;  // a negative scale's sign goes to Q: the largest score is then the largest product
+  // What follows from the lane is formed where it is used, again and again: kept over the pages it would spill, and a
+  // spill's reload waits for the DMAs.
+  auto thread = [] {
+    uint32_t x = threadIdx.x;
+    asm volatile("" : "+v"(x));
+    return x;
+  };
 
   while (u < u1) {
-    // What follows from the lane is formed where it is used, again and again: kept over the pages it would spill, and a
-    // spill's reload waits for the DMAs.
-    auto thread = [] {
-      uint32_t x = threadIdx.x;
-      asm volatile("" : "+v"(x));
-      return x;
-    };
     uint32_t slot = t.slots - 1 - run, tile_u = 0;  // one tile each: the last, longest ones first
     Tile tile;
     if constexpr (RUNS) {
@@ -74,11 +83,11 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_wide_kernel(KvArgs a, At
       return;
     }
     uint32_t row, head;
-    pair_at(t, tile, kvh, min(32 * wave + (thread() & 31), tile.pairs - 1), row, head);
+    pair_at(t, tile, kvh, min(32 * group + (thread() & 31), tile.pairs - 1), row, head);
     const uint32_t seen = seen_by(a, row);
     const uint32_t wmost = wave_max_u32(seen), wleast = ~wave_max_u32(~seen);
     if ((thread() & 63) == 0) seen_most[wave] = wmost;
-    // Q: dims 32 c + 16 f + 8 e .. + 7 of pair r
+    // Q: dims 32 x + 16 f + 8 e .. + 7 of pair r
     h8 q[2 * C];
     {
       const _Float16* qp = t.q + (size_t)row * t.ldq + head * D + 16 * (thread() >> 5 & 1);
@@ -93,7 +102,8 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_wide_kernel(KvArgs a, At
       }
     }
     __syncthreads();
-    const uint32_t most = __builtin_amdgcn_readfirstlane(max(max(seen_most[0], seen_most[1]), max(seen_most[2], seen_most[3])));
+    const uint32_t most =
+        __builtin_amdgcn_readfirstlane(max(max(seen_most[0], seen_most[1]), max(seen_most[2], seen_most[3])));
     const uint32_t npages = pages_of(a, most);
     const uint32_t b0 = u - tile_u, b1 = RUNS ? min(npages, u1 - tile_u) : npages;
     if (RUNS && b1 <= b0) return;  // positions that changed under the call
@@ -101,24 +111,29 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_wide_kernel(KvArgs a, At
     const scalar_words table = (scalar_words)(a.table + (size_t)tile.seq * a.ld_table);
     auto page_id = [&](uint32_t b) -> uint32_t { return b < a.ld_table ? table[b] : 0xffffffffu; };
     auto record = [&](uint32_t id) { return a.pool + (id < a.pages ? id : 0) * a.page_bytes; };
-    // a page's K and V into buffer buf: 1 KB a wave and DMA. The swizzles of the i-th 4 KB are the first's, but for D = 256,
-    // where K's odd ones have another bit of the key.
-    auto stage = [&](uint32_t id, uint32_t buf) {
-      const uint8_t* const kp = record(id) + kv_k_at<D>(kvh);
-      const uint8_t* const vp = record(id) + kv_v_at<D>(kvh, a.kv_heads);
+    // a page's K, V and scales into place `to` (0 .. 3), in kPieces DMAs of 1 KB a wave; the scales by one wave
+    auto stage_piece = [&](const uint8_t* rec, uint32_t to, uint32_t i) {
       constexpr uint32_t kRow = D / 16;  // chunks of a token
-      const uint32_t lane = thread() & 63;
-      const uint32_t tok = wave * (1024 / D) + lane / kRow, dim = wave * 16 + lane / 4;
-      const uint32_t kx = tok * D + (lane % kRow ^ k_key<D>(tok)) * 16, vx = dim * 64 + (lane % 4 ^ (dim >> 1 & 3)) * 16;
-#pragma unroll
-      for (uint32_t i = 0; i < kBytes / 4096; ++i) {
-        const uint32_t at = i * 4096 + wave * 1024;
-        dma16(lds0 + buf * kBytes + at, D == 256 && i % 2 ? kx ^ 128 : kx, kp + i * 4096);
-        dma16(lds0 + (2 + buf) * kBytes + at, vx, vp + i * 4096);
+      const uint32_t lane = thread() & 63, at = (8 * i + wave) * 1024;
+      if (at < kBytes) {
+        const uint32_t tok = at / D + lane / kRow, x = lane % kRow ^ k_key<D>(tok);
+        dma16(lds0 + to * 2 * kBytes + at, tok * D + x * 16, rec + kv_k_at<D>(kvh));
+      } else {
+        const uint32_t dim = (at - kBytes) / 64 + lane / 4, x = lane % 4 ^ (dim >> 1 & 3);
+        dma16(lds0 + to * 2 * kBytes + at, dim * 64 + x * 16, rec + kv_v_at<D>(kvh, a.kv_heads));
       }
-      if (wave == 0 && lane < 2) dma16(scales0 + buf * 1024, lane * 16, record(id) + kv_scale_at<D>(kvh, a.kv_heads));
+    };
+    auto stage_scales = [&](const uint8_t* rec, uint32_t to) {
+      const uint32_t lane = thread() & 63;
+      if (wave == to && lane < 2) dma16(scales0 + to * 1024, lane * 16, rec + kv_scale_at<D>(kvh, a.kv_heads));
+    };
+    auto stage = [&](uint32_t id, uint32_t to) {
+      stage_scales(record(id), to);
+#pragma unroll
+      for (uint32_t i = 0; i < kPieces; ++i) stage_piece(record(id), to, i);
     };
 
+    // O: o[i] holds dims 32 i' .., i' = i for half 0, i ^ DT / 2 for half 1: what a wave keeps at the end comes first
     f16v o[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i)
@@ -127,129 +142,175 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_wide_kernel(KvArgs a, At
     float m = -INFINITY, l = 0.f;
     float vref = 0x1p-100f, inv_vref = 0x1p100f;
 
-    uint32_t id = b0 < b1 ? page_id(b0) : 0;
-    if (b0 < b1) stage(id, 0);
+    auto id_of = [&](uint32_t b) { return b < b1 ? page_id(b) : 0; };
+    uint32_t id0 = id_of(b0), id1 = id_of(b0 + 1), id2 = id_of(b0 + 2), id3 = id_of(b0 + 3);  // of pages b .. b + 3
+    if (b0 < b1) stage(id0, 0);
+    if (b0 + 1 < b1) stage(id1, 1);
+    if (b0 + 2 < b1) stage(id2, 2);
     wait_vm<0>();
 #pragma unroll
     for (int x = 0; x < 2 * C; ++x) tie(q[x]);  // no wait for Q in the loop: it would wait for the DMAs too
     __syncthreads();
-    for (uint32_t b = b0, buf = 0; b < b1; ++b, buf ^= 1) {
-      const uint32_t next = b + 1 < b1 ? page_id(b + 1) : 0;
-      if (b + 1 < b1) stage(next, buf ^ 1);  // into the buffer every wave left before the last barrier
-      const bool bad = id >= a.pages;
-      char* const vb = lds + (2 + buf) * kBytes;
-      if (b * kKvPage + (kKvPage - 1) >= most) {  // bytes behind the last seen token may be anything
-        const uint32_t have = most % kKvPage;
-        for (uint32_t i = thread(); i < D * 4; i += 256) {
-          const uint32_t dim = i / 4, x = i % 4, left = have > 16 * x ? min(have - 16 * x, 16u) : 0;
-          u4* const at = (u4*)(vb + dim * 64 + (x ^ (dim >> 1 & 3)) * 16);
-          u4 v = *at;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int n = (int)left - 4 * w;
-            v[w] &= n >= 4 ? ~0u : n <= 0 ? 0u : (1u << 8 * n) - 1u;
-          }
-          *at = v;
-        }
-        __syncthreads();
-      }
-      if (b * kKvPage < wmost) {
-#pragma unroll 1
-        for (uint32_t T = 0; T < 2; ++T) {
-          const uint32_t lane = thread() & 63, r = lane & 31, f = lane >> 5;
-          // the key of row m = 8 x + 4 y + i is token 16 (2 T + y) + 4 x + i
-          const uint32_t tok = 16 * (2 * T + (r >> 2 & 1)) + 4 * (r >> 3) + (r & 3);
-          const char* const kb = lds + buf * kBytes + tok * D;
-          uint32_t sw = (f ^ k_key<D>(tok)) * 16;  // chunk 2 x + f of the token lies at byte 32 x ^ sw
-          asm volatile("" : "+v"(sw));             // formed here: hoisted addresses would spill
-          f16v st;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) st[e] = 0.f;
-          // reads run two ahead of the products; the barriers keep the compiler from moving them to their use
-          u4 kf[3];
-#pragma unroll
-          for (int x = 0; x < 2; ++x) kf[x] = *(const u4*)(kb + ((32 * x) ^ sw));
-#pragma unroll
-          for (int x = 0; x < C; ++x) {
-            if (x + 2 < C) kf[(x + 2) % 3] = *(const u4*)(kb + ((32 * (x + 2)) ^ sw));
-            __builtin_amdgcn_sched_barrier(0);
-            const u4 k = kf[x % 3];
-            st = mfma32(numbers<INT8>(k[0], k[1]), q[2 * x], st);
-            st = mfma32(numbers<INT8>(k[2], k[3]), q[2 * x + 1], st);
-          }
-          const char* const vt = vb + r * 64 + ((2 * T + f) ^ (r >> 1 & 3)) * 16;  // 32 dims on: 2,048 bytes, the same swizzle
-          u4 vf[3];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) vf[i] = *(const u4*)(vt + 2048 * i);
-          const float ks = scales[buf][2 * T + f];
-          float vs = scales[buf][4 + 2 * T + f];
-          const float cs = c * (bad ? NAN : ks);
-          float unit = cs;  // scores are st * unit, or st where a mask has scaled them
-          bool blind = false;
-          if (b * kKvPage + (kKvPage - 1) >= wleast) {  // some pair does not see all of the page
-            const uint32_t tok0 = b * kKvPage + 16 * (2 * T + f);  // below 2^32, as seen is
-            const uint32_t mine = seen > tok0 ? min(seen - tok0, 16u) : 0;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) st[i] = i < (int)mine ? st[i] * cs : -INFINITY;
-            unit = 1.0f;
-            blind = mine == 0;
-            if (tok0 >= most) vs = 0.f;
-          }
-          float bm = st[0];
-#pragma unroll
-          for (int i = 1; i < 16; ++i) bm = fmaxf(bm, st[i]);
-          bm = max_halves(bm * unit);
-          // the same in every lane: kept in scalar registers
-          const float vm = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(max_halves(vs))));
-          if (__any(bm > m + kLazy) || vm > vref) {
-            const float mnew = bm > m + kLazy ? bm : m;
-            const float alpha = state_weight(m, mnew);
-            const float vnew = fmaxf(vref, vm);
-            l *= alpha;
-            m = mnew;
-            const float both = alpha * (vref / vnew);
-            vref = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(vnew)));
-            inv_vref = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(1.0f / vnew)));
-#pragma unroll
-            for (int i = 0; i < DT; ++i) o[i] *= both;
-          }
-          const float mref = m == -INFINITY ? 0.f : m;
-          const float ratio = blind ? 0.f : vs * inv_vref;
-          h8 p[2];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float w = __builtin_amdgcn_exp2f(fmaf(st[i], unit, -mref));
-            l += w;
-            p[i / 8][i % 8] = (_Float16)(w * ratio);
-          }
-#pragma unroll
-          for (int i = 0; i < DT; ++i) {
-            if (i + 2 < DT) vf[(i + 2) % 3] = *(const u4*)(vt + 2048 * (i + 2));
-            __builtin_amdgcn_sched_barrier(0);
-            const u4 v = vf[i % 3];
-            o[i] = mfma32(numbers<INT8>(v[0], v[1]), p[0], o[i]);
-            o[i] = mfma32(numbers<INT8>(v[2], v[3]), p[1], o[i]);
-          }
-        }
-      }
-      id = next;
-      wait_vm<0>();
+    // One barrier a page. Half 0 meets it before the page's first products, half 1 between the page's softmax and its
+    // products with V, a page's work ahead: so of the two waves of a SIMD one is at its products while the other is at its
+    // softmax. At barrier b pages up to b + 1 have landed and page b - 1 is done with: behind it page b + 3 is sent for.
+    auto meet_at = [&](uint32_t b) {
+      if (b + 2 < b1)
+        wait_vm<kPieces>();  // all but page b + 2
+      else
+        wait_vm<0>();
       __syncthreads();
+    };
+    for (uint32_t b = b0; b < b1; ++b) {
+      const uint32_t at = (b - b0) & 3;
+      if (T == 0) {
+        if (b * kKvPage + (kKvPage - 1) >= most) {  // bytes behind the last seen token may be anything
+          char* const vb = lds + (at * 2 + 1) * kBytes;
+          const uint32_t have = most % kKvPage;
+          for (uint32_t i = thread(); i < D * 4; i += 256) {
+            const uint32_t dim = i / 4, x = i % 4, left = have > 16 * x ? min(have - 16 * x, 16u) : 0;
+            u4* const to = (u4*)(vb + dim * 64 + (x ^ (dim >> 1 & 3)) * 16);
+            u4 v = *to;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const int n = (int)left - 4 * w;
+              v[w] &= n >= 4 ? ~0u : n <= 0 ? 0u : (1u << 8 * n) - 1u;
+            }
+            *to = v;
+          }
+        }
+        meet_at(b);
+        if (b + 3 < b1) stage(id3, (at + 3) & 3);
+      }
+      const bool on = b * kKvPage + 32 * T < wmost;  // some pair of the wave sees the half
+      h8 p[2];
+      if (on) {
+        const bool bad = id0 >= a.pages;
+        const uint32_t lane = thread() & 63, r = lane & 31, f = lane >> 5;
+        // the key of row m = 8 x + 4 y + i is token 16 (2 T + y) + 4 x + i
+        const uint32_t tok = 16 * (2 * T + (r >> 2 & 1)) + 4 * (r >> 3) + (r & 3);
+        const char* const kb = lds + at * 2 * kBytes + tok * D;
+        uint32_t sw = (f ^ k_key<D>(tok)) * 16;  // chunk 2 x + f of the token lies at byte 32 x ^ sw
+        asm volatile("" : "+v"(sw));             // formed here: hoisted addresses would spill
+        __builtin_amdgcn_s_setprio(1);  // the wave at its products goes first: 37 pages 84 us against 76
+        f16v st;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) st[e] = 0.f;
+        // reads run kAhead products ahead; the barriers keep the compiler from moving them to their use
+        u4 kf[kAhead + 1];
+#pragma unroll
+        for (int x = 0; x < (kAhead < C ? kAhead : C); ++x) kf[x] = *(const u4*)(kb + ((32 * x) ^ sw));
+#pragma unroll
+        for (int x = 0; x < C; ++x) {
+          if (x + kAhead < C) kf[(x + kAhead) % (kAhead + 1)] = *(const u4*)(kb + ((32 * (x + kAhead)) ^ sw));
+          __builtin_amdgcn_sched_barrier(0);
+          const u4 k = kf[x % (kAhead + 1)];
+          st = mfma32(numbers<INT8>(k[0], k[1]), q[2 * x], st);
+          st = mfma32(numbers<INT8>(k[2], k[3]), q[2 * x + 1], st);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        const float ks = scales[at][2 * T + f];
+        float vs = scales[at][4 + 2 * T + f];
+        const float cs = c * (bad ? NAN : ks);
+        float unit = cs;  // scores are st * unit, or st where a mask has scaled them
+        bool blind = false;
+        if (b * kKvPage + 32 * T + 31 >= wleast) {  // some pair does not see all of the half
+          const uint32_t tok0 = b * kKvPage + 16 * (2 * T + f);  // below 2^32, as seen is
+          const uint32_t mine = seen > tok0 ? min(seen - tok0, 16u) : 0;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) st[i] = i < (int)mine ? st[i] * cs : -INFINITY;
+          unit = 1.0f;
+          blind = mine == 0;
+          if (tok0 >= most) vs = 0.f;
+        }
+        float bm = st[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) bm = fmaxf(bm, st[i]);
+        bm = max_halves(bm * unit);
+        // the same in every lane: kept in scalar registers
+        const float vm = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(max_halves(vs))));
+        if (__any(bm > m + kLazy) || vm > vref) {
+          const float mnew = bm > m + kLazy ? bm : m;
+          const float alpha = state_weight(m, mnew);
+          const float vnew = fmaxf(vref, vm);
+          l *= alpha;
+          m = mnew;
+          const float both = alpha * (vref / vnew);
+          vref = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(vnew)));
+          inv_vref = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(1.0f / vnew)));
+#pragma unroll
+          for (int i = 0; i < DT; ++i) o[i] *= both;
+        }
+        const float mref = m == -INFINITY ? 0.f : m;
+        const float ratio = blind ? 0.f : vs * inv_vref;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float w = __builtin_amdgcn_exp2f(fmaf(st[i], unit, -mref));
+          l += w;
+          p[i / 8][i % 8] = (_Float16)(w * ratio);
+        }
+      }
+      if (T == 1) meet_at(b);
+      if (on) {
+        // V: 32 dims on are 2,048 bytes, with the same swizzle
+        const uint32_t lane = thread() & 63, r = lane & 31, f = lane >> 5;
+        const char* const vt = lds + (at * 2 + 1) * kBytes + r * 64 + ((2 * T + f) ^ (r >> 1 & 3)) * 16;
+        const char* const v0 = vt + T * (kBytes / 2);
+        const char* const v1 = vt + (1 - T) * (kBytes / 2) - kBytes / 2;
+        auto read_v = [&](int i) { return *(const u4*)((i < DT / 2 ? v0 : v1) + 2048 * i); };
+        __builtin_amdgcn_s_setprio(1);
+        u4 vf[kAhead + 1];
+#pragma unroll
+        for (int i = 0; i < (kAhead < DT ? kAhead : DT); ++i) vf[i] = read_v(i);
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+          if (i + kAhead < DT) vf[(i + kAhead) % (kAhead + 1)] = read_v(i + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
+          const u4 v = vf[i % (kAhead + 1)];
+          o[i] = mfma32(numbers<INT8>(v[0], v[1]), p[0], o[i]);
+          o[i] = mfma32(numbers<INT8>(v[2], v[3]), p[1], o[i]);
+        }
+      }
+      if (T == 1 && b + 3 < b1) stage(id3, (at + 3) & 3);
+      __builtin_amdgcn_s_setprio(0);
+      id0 = id1, id1 = id2, id2 = id3, id3 = id_of(b + 4);
     }
+    __syncthreads();  // the states go where the pages lie
 
+    // The halves' states meet: each wave keeps its first o's and gives its partner the rest.
+    const uint32_t lane = thread() & 63, r = lane & 31, f = lane >> 5;
+    f4* const xo = (f4*)lds;
     l = sum_halves(l);
-    const uint32_t r = thread() & 31, f = thread() >> 5 & 1;
-    if (32 * wave + r < tile.pairs) {
+    if (f == 0) meet[wave * 32 + r] = f4{m, l, vref, 0.f};
+#pragma unroll
+    for (int i = 0; i < DT / 2 * 4; ++i) {
+      const f16v& v = o[DT / 2 + i / 4];
+      const int e = 4 * (i % 4);
+      xo[(wave * (DT / 2 * 4) + i) * 64 + lane] = f4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+    }
+    __syncthreads();
+    if (32 * group + r < tile.pairs) {
+      const f4 other = meet[(wave ^ 4) * 32 + r];
+      const float top = fmaxf(m, other[0]);
+      const float wm = state_weight(m, top), wo = state_weight(other[0], top);
+      // (a NaN sum stays: a state without a score has weight 0 and, but for NaN, the sum 0)
+      const float lt = (m == -INFINITY ? l : l * wm) + (other[0] == -INFINITY ? other[1] : other[1] * wo);
+      const float fm = wm * vref, fo = wo * other[2];
+      auto merged = [&](int i) {
+        const f4 po = xo[((wave ^ 4) * (DT / 2 * 4) + i) * 64 + lane];
+        f4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = fmaf(po[e], fo, o[i / 4][4 * (i % 4) + e] * fm);
+        return v;
+      };
+      const uint32_t d0 = T * (D / 2) + 4 * f;  // dims d0 + 32 (i / 4) + 8 (i % 4) ..
       if (whole) {
-        pair_at(t, tile, kvh, 32 * wave + r, row, head);
-        const float factor = over_sum(l) * vref;
+        pair_at(t, tile, kvh, 32 * group + r, row, head);
+        const float factor = over_sum(lt);
         auto store = [&](auto gate) {
 #pragma unroll
-          for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              store_out<decltype(gate)::value>(t, row, head * D + 32 * i + 8 * x + 4 * f,
-                                               f4{o[i][4 * x], o[i][4 * x + 1], o[i][4 * x + 2], o[i][4 * x + 3]}, factor);
+          for (int i = 0; i < DT / 2 * 4; ++i)
+            store_out<decltype(gate)::value>(t, row, head * D + d0 + 32 * (i / 4) + 8 * (i % 4), merged(i), factor);
         };
         if (t.gate)
           store(std::true_type{});
@@ -257,18 +318,14 @@ __global__ __launch_bounds__(256, 2) void kv8_attention_wide_kernel(KvArgs a, At
           store(std::false_type{});
       } else {
         float* const state = state_of<D, kKvWideTile>(t, kvh, run, u == first_u ? 0 : 1);
-        float* const at = state + (32 * wave + r) * D + 4 * f;
+        float* const to = state + (32 * group + r) * D + d0;
 #pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            *(f4*)(at + 32 * i + 8 * x) =
-                f4{o[i][4 * x], o[i][4 * x + 1], o[i][4 * x + 2], o[i][4 * x + 3]} * vref;
-        if (f == 0) *(f2*)(state + kKvWideTile * D + 2 * (32 * wave + r)) = f2{m, l};
+        for (int i = 0; i < DT / 2 * 4; ++i) *(f4*)(to + 32 * (i / 4) + 8 * (i % 4)) = merged(i);
+        if (T == 0 && f == 0) *(f2*)(state + kKvWideTile * D + 2 * (32 * group + r)) = f2{top, lt};
       }
     }
     if constexpr (!RUNS) return;
-    __syncthreads();  // seen_most is written again
+    __syncthreads();  // the next tile's pages go where the states lay
     u = tile_u + b1;
   }
 }
@@ -278,7 +335,7 @@ template <int D>
 void wide_kernels(const KvArgs& a, const AttnArgs& t, bool int8, hipStream_t s) {
   const dim3 grid(a.kv_heads * (t.runs ? t.runs : t.slots));
   auto go = [&](auto i8, auto runs) {
-    hipLaunchKernelGGL((kv8_attention_wide_kernel<D, decltype(i8)::value, decltype(runs)::value>), grid, dim3(256), 0, s,
+    hipLaunchKernelGGL((kv8_attention_wide_kernel<D, decltype(i8)::value, decltype(runs)::value>), grid, dim3(512), 0, s,
                        a, t);
   };
   auto with = [&](auto i8) { t.runs ? go(i8, std::true_type{}) : go(i8, std::false_type{}); };
