@@ -164,7 +164,7 @@ int dh_kv8_append(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, uint32_t
   rc = check_rows("kv8_append", "k", k, ldk, dtype, wide);
   if (rc == DH_OK) rc = check_rows("kv8_append", "v", v, ldv, dtype, wide);
   if (rc != DH_OK) return rc;
-  if ((uint64_t)batch->rows / DH_KV8_PAGE + 2 * (uint64_t)batch->seqs > INT32_MAX)
+  if ((uint64_t)batch->rows / DH_KV8_BLOCK + 2 * (uint64_t)batch->seqs > INT32_MAX)
     return fail(DH_EINVAL, "kv8_append: %u sequences exceed one launch; split the call", batch->seqs);
   if (!ctx) return fail(DH_EINVAL, "kv8_append: null context");
   if (batch->rows && batch->seqs && (!k || !v)) return fail(DH_EINVAL, "kv8_append: null pointer");

@@ -4,8 +4,7 @@
 //           lane). The angle position * inv_freq is a product of a whole number and an fp32 one: exact in 64 bits up
 //           to positions of 2^29, where in 32 bits it is off by half a turn's fraction already at 10^5. It is formed
 //           and reduced to half turns in 64 bits, once per row and pair, and shared by the heads through LDS.
-//   append  codes K and V rows into pages. A wave takes one block (16 tokens of one head, K or V), so the largest
-//           magnitude, the scale, the earlier tokens' new codes and the stores need no other wave.
+//   append  codes K and V rows into pages, a workgroup a block (16 tokens of one head, K or V).
 //   copy    moves whole pages, 16 bytes a lane.
 //
 // All three are bound by memory: each value is read once and written once.
@@ -300,9 +299,9 @@ __device__ __forceinline__ uint32_t recode4(uint32_t u, float ratio) {
   return code4<INT8>(v[0] * ratio, v[1] * ratio, v[2] * ratio, v[3] * ratio);
 }
 
-// Largest magnitude of a wave's values and whether all are finite, then the block's scale: `keep` tokens stay with theirs.
-template <bool INT8, int N>
-__device__ __forceinline__ float new_scale(const float* x, bool keep, float before) {
+// What a wave's values say to its block: their largest magnitude, NaN where one is not finite.
+template <int N>
+__device__ __forceinline__ float wave_amax(const float* x) {
   float amax = 0.f;
   bool finite = true;
 #pragma unroll
@@ -310,173 +309,146 @@ __device__ __forceinline__ float new_scale(const float* x, bool keep, float befo
     amax = fmaxf(amax, fabsf(x[i]));
     finite = finite && fabsf(x[i]) < INFINITY;
   }
-  const float s = block_scale<INT8>(reduce<64>(amax, [](float a, float b) { return fmaxf(a, b); }));
-  if (!__all(finite) || (keep && before != before)) return NAN;
-  return keep ? fmaxf(s, before) : s;
+  amax = reduce<64>(amax, [](float a, float b) { return fmaxf(a, b); });
+  return __all(finite) ? amax : NAN;
 }
 
-// A workgroup is one page of one sequence x one head x K or V, a wave one block of the page.
+// A workgroup is one block (16 tokens of one head, K or V). K: a wave takes four tokens, 4 dims a lane. V: a thread takes
+// one dim of 16, 8 or 4 tokens (D = 256, 128, 64), which are consecutive bytes. The waves meet once, over the largest
+// magnitude. With a wave per block, and so four times fewer waves with four times the work each, 2,307 rows took 18.7 us
+// against XX.
 template <typename T, int D, bool INT8>
 __global__ __launch_bounds__(256) void kv8_append_kernel(KvArgs a, const void* __restrict__ k, uint32_t ldk,
                                                          const void* __restrict__ v, uint32_t ldv, RopeArgs rope) {
-  constexpr int W = D / 4;        // lanes of a key
-  constexpr int TP = 64 / W;      // keys a wave reads at once
-  constexpr int P = kKvBlock / TP;  // passes over a block's keys
-  __shared__ double cs[4][4][128][2];
+  extern __shared__ __attribute__((aligned(16))) double angles[];  // (cos, sin) [4 waves][4 tokens][rot / 2]
+  __shared__ float amax[4];
   const uint32_t head = blockIdx.y % a.kv_heads;
   const bool is_v = blockIdx.y >= a.kv_heads;
   uint32_t r0, r1;
-  const uint32_t s = kv_find_seq(a.row0, a.seqs, a.rows, blockIdx.x, 1, kKvPage, 2, r0, r1);
+  const uint32_t s = kv_find_seq(a.row0, a.seqs, a.rows, blockIdx.x, 1, kKvBlock, 2, r0, r1);
   if (s >= a.seqs || r1 <= r0) return;
   const uint64_t p0 = a.qpos[r0], p1 = p0 + (r1 - r0);  // the tokens p0 .. p1 - 1 are new
-  const uint64_t page = p0 / kKvPage + (blockIdx.x - (r0 / kKvPage + 2 * s));
-  const uint32_t lane = threadIdx.x & 63, block = threadIdx.x >> 6;
-  const uint64_t t0 = page * kKvPage + block * kKvBlock;  // the block's first token
-  if (p0 == 0xffffffffu || page >= a.ld_table || t0 >= p1 || t0 + kKvBlock <= p0) return;
+  const uint64_t t0 = (p0 / kKvBlock + (blockIdx.x - (r0 / kKvBlock + 2 * s))) * kKvBlock;  // the block's first token
+  const uint64_t page = t0 / kKvPage;
+  if (p0 == 0xffffffffu || page >= a.ld_table || t0 >= p1) return;
   const uint32_t id = a.table[(size_t)s * a.ld_table + page];
   if (id >= a.pages) return;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, block = (uint32_t)(t0 % kKvPage) / kKvBlock;
   uint8_t* const rec = a.pool + id * a.page_bytes;
   float* const scale = (float*)(rec + kv_scale_at<D>(head, a.kv_heads)) + (is_v ? 4 : 0) + block;
-  const uint32_t kept = p0 > t0 ? (uint32_t)(p0 - t0) : 0;                      // earlier tokens of the block
+  const uint32_t kept = p0 > t0 ? (uint32_t)(p0 - t0) : 0;                    // earlier tokens of the block
   const uint32_t end = p1 < t0 + kKvBlock ? (uint32_t)(p1 - t0) : kKvBlock;  // its new tokens are kept .. end - 1
   const float before = kept ? *scale : 0.f;
   const size_t row = r0 + (size_t)(t0 - p0);  // the row of the block's token 0 (wraps below zero before row r0)
+  auto row_of = [&](uint32_t t) { return row + min(max(t, kept), end - 1); };  // one of the call's in place of others
+
+  // the block's scale, once the waves have left what they say
+  auto block_scale_now = [&](float mine) {
+    if (lane == 0) amax[wave] = mine;
+    __syncthreads();
+    const float a0 = amax[0], a1 = amax[1], a2 = amax[2], a3 = amax[3];
+    const float sum = a0 + a1 + a2 + a3;  // NaN where one is
+    const float fresh = block_scale<INT8>(fmaxf(fmaxf(a0, a1), fmaxf(a2, a3)));
+    const float sc = sum != sum || (kept && before != before) ? NAN : kept ? fmaxf(fresh, before) : fresh;
+    if (tid == 0) *scale = sc;
+    return sc;
+  };
 
   if (is_v) {
-    constexpr int C = D / 64;  // dims of a lane, all 16 tokens
-    const uint32_t d = lane * C;
-    Raw<T, C> raw[kKvBlock];
+    constexpr int N = kKvBlock * D / 256;  // tokens of a thread
+    const uint32_t d = tid % D, tok = tid / D * N;
+    Raw<T, 1> raw[N];
 #pragma unroll
-    for (uint32_t t = 0; t < kKvBlock; ++t)  // a row of the call in place of those that are none of it
-      raw[t].load(v, (row + min(max(t, kept), end - 1)) * ldv + head * D + d);
-    uint8_t* const at = rec + kv_v_at<D>(head, a.kv_heads) + (size_t)d * kKvPage + block * kKvBlock;
-    u4 old[C];
+    for (int t = 0; t < N; ++t) raw[t].load(v, row_of(tok + t) * ldv + head * D + d);
+    struct alignas(N) Words {
+      uint32_t w[N / 4];
+    };
+    Words* const at = (Words*)(rec + kv_v_at<D>(head, a.kv_heads) + (size_t)d * kKvPage + block * kKvBlock + tok);
+    Words old{};
+    if (kept) old = *at;
+    float x[N];
 #pragma unroll
-    for (int c = 0; c < C; ++c) old[c] = kept ? *(const u4*)(at + c * kKvPage) : u4{0, 0, 0, 0};
-    float x[kKvBlock][C];
+    for (int t = 0; t < N; ++t) x[t] = tok + t >= kept && tok + t < end ? raw[t][0] : 0.f;
+    const float sc = block_scale_now(wave_amax<N>(x));
+    const float inv = 1.0f / sc, ratio = before / sc;
+    Words out;
 #pragma unroll
-    for (uint32_t t = 0; t < kKvBlock; ++t)
+    for (int w = 0; w < N / 4; ++w) {
+      float q[4];
 #pragma unroll
-      for (int c = 0; c < C; ++c) x[t][c] = t >= kept && t < end ? raw[t][c] : 0.f;
-    const float sc = new_scale<INT8, kKvBlock * C>(&x[0][0], kept != 0, before);
-    const float inv = 1.0f / sc;
-    if (lane == 0) *scale = sc;
-    if (kept) {
-      if (sc > before) {
-        const float ratio = before / sc;
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) old[c][w] = recode4<INT8>(old[c][w], ratio);
-      }
+      for (int i = 0; i < 4; ++i) q[i] = sc == sc ? scaled<INT8>(x[4 * w + i], sc, inv) : 0.f;
+      const int stay = (int)kept - (int)tok - 4 * w;  // bytes of tokens that stay
+      const uint32_t m = stay >= 4 ? ~0u : stay <= 0 ? 0u : (1u << 8 * stay) - 1u;
+      uint32_t o = old.w[w];
+      if (kept && sc > before) o = recode4<INT8>(o, ratio);
+      out.w[w] = (o & m) | (code4<INT8>(q[0], q[1], q[2], q[3]) & ~m);
     }
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      u4 out;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        float q[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = sc == sc ? scaled<INT8>(x[4 * w + i][c], sc, inv) : 0.f;
-        const int stay = (int)kept - 4 * w;  // bytes of tokens that stay
-        const uint32_t m = stay >= 4 ? ~0u : stay <= 0 ? 0u : (1u << 8 * stay) - 1u;
-        out[w] = (old[c][w] & m) | (code4<INT8>(q[0], q[1], q[2], q[3]) & ~m);
-      }
-      *(u4*)(at + c * kKvPage) = out;
-    }
+    *at = out;
     return;
   }
 
-  // K: pass n holds token n TP + lane / W, 4 dims a lane
+  constexpr int W = D / 4;   // lanes of a key
+  constexpr int TP = 64 / W;  // keys a wave reads at once
+  constexpr int P = 4 / TP;   // passes over its four: pass n holds token 4 wave + n TP + lane / W
   const uint32_t d = 4 * (lane % W);
-  auto token = [&](int n) { return n * TP + lane / W; };
-  auto source = [&](int n) { return (row + min(max(token(n), kept), end - 1)) * ldk + head * D; };
+  auto token = [&](int n) { return 4 * wave + n * TP + lane / W; };
   Raw<T, 4> raw[P];
 #pragma unroll
-  for (int n = 0; n < P; ++n) raw[n].load(k, source(n) + d);
-  // the block as it was, 16 bytes a lane
-  constexpr int B = D / 64;
+  for (int n = 0; n < P; ++n) raw[n].load(k, row_of(token(n)) * ldk + head * D + d);
+  // the block as it was, 16 bytes a thread
   uint8_t* const base = rec + kv_k_at<D>(head) + (size_t)block * kKvBlock * D;
-  u4 old[B];
-#pragma unroll
-  for (int j = 0; j < B; ++j) old[j] = kept ? *(const u4*)(base + j * 1024 + lane * 16) : u4{0, 0, 0, 0};
+  u4 old = u4{0, 0, 0, 0};
+  const bool stays = tid * 16 / D < kept;  // (a thread's 16 bytes are one token's)
+  if (stays) old = *(const u4*)(base + tid * 16);
   float x[P][4];
-  if (rope.inv_freq) {
+#pragma unroll
+  for (int n = 0; n < P; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[n][i] = raw[n][i];
+  if (rope.inv_freq && 4 * wave < end && 4 * wave + 4 > kept) {
     Turn<double> turn;
     turn.init(rope, lane % W, D, rope.add_one ? 1.0 : 0.0);
-    auto pass = [&](int n) {
-      float own[4];
+    const uint32_t pairs = rope.rot / 2;
+    double(*const cs)[2] = (double(*)[2])angles + (size_t)wave * 4 * pairs;
+    for (uint32_t i = lane; i < 4 * pairs; i += 64) {
+      const uint32_t pair = i % pairs, t = 4 * wave + i / pairs;
+      if (t < kept || t >= end) continue;
+      double sn, c;
+      sincospi(half_turns((double)(t0 + t), rope.inv_freq[pair]), &sn, &c);
+      cs[i][0] = c * (double)rope.amp;
+      cs[i][1] = sn * (double)rope.amp;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // this wave's own reads follow
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) own[i] = raw[n][i];
-      const double inv = rope.norm_w ? norm_factor<W, double>(own, D, rope.eps) : 1.0;
+    for (int n = 0; n < P; ++n) {
+      if (4 * wave + n * TP >= end || 4 * wave + n * TP + TP <= kept) continue;
+      const double inv = rope.norm_w ? norm_factor<W, double>(x[n], D, rope.eps) : 1.0;
       double y[4];
-      turn4<T, W, double>(own, k, source(n), rope, turn, inv, cs[block][token(n) % 4], y);
+      turn4<T, W, double>(x[n], k, row_of(token(n)) * ldk + head * D, rope, turn, inv, cs + token(n) % 4 * pairs, y);
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[n][i] = (float)y[i];
-    };
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {  // four tokens share a table of angles
-#pragma unroll
-      for (int j = 0; j < P / 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[g * (P / 4) + j][i] = 0.f;
-      if (4u * g >= end || 4u * g + 4 <= kept) continue;
-      __builtin_amdgcn_wave_barrier();
-      const uint32_t pairs = rope.rot / 2;
-      for (uint32_t i = lane; i < 4 * pairs; i += 64) {
-        const uint32_t pair = i % pairs, t = i / pairs;
-        if (4 * g + t < kept || 4 * g + t >= end) continue;
-        double sn, c;
-        sincospi(half_turns((double)(t0 + 4 * g + t), rope.inv_freq[pair]), &sn, &c);
-        cs[block][t][pair][0] = c * (double)rope.amp;
-        cs[block][t][pair][1] = sn * (double)rope.amp;
-      }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // this wave's own reads follow
-      __builtin_amdgcn_wave_barrier();
-      if (4u * g >= kept && 4u * g + 4 <= end) {
-#pragma unroll
-        for (int j = 0; j < P / 4; ++j) pass(g * (P / 4) + j);
-      } else {  // a new token or two: only the passes that hold them
-#pragma unroll
-        for (int j = 0; j < P / 4; ++j) {
-          const uint32_t n = g * (P / 4) + j;
-          if (n * TP < end && n * TP + TP > kept) pass(n);
-        }
-      }
     }
-  } else {
-#pragma unroll
-    for (int n = 0; n < P; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[n][i] = raw[n][i];
   }
 #pragma unroll
-  for (int n = 0; n < P; ++n) {
-    const uint32_t t = token(n);
+  for (int n = 0; n < P; ++n)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[n][i] = t >= kept && t < end ? x[n][i] : 0.f;
-  }
-  const float sc = new_scale<INT8, P * 4>(&x[0][0], kept != 0, before);
+    for (int i = 0; i < 4; ++i) x[n][i] = token(n) >= kept && token(n) < end ? x[n][i] : 0.f;
+  const float sc = block_scale_now(wave_amax<P * 4>(&x[0][0]));
   const float inv = 1.0f / sc;
-  if (lane == 0) *scale = sc;
-  if (kept && sc > before) {
+  if (stays && sc > before) {
     const float ratio = before / sc;
+    u4 now;
 #pragma unroll
-    for (int j = 0; j < B; ++j) {
-      if ((j * 1024 + lane * 16) / D >= kept) continue;
-      u4 now;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) now[w] = recode4<INT8>(old[j][w], ratio);
-      *(u4*)(base + j * 1024 + lane * 16) = now;
-    }
+    for (int w = 0; w < 4; ++w) now[w] = recode4<INT8>(old[w], ratio);
+    *(u4*)(base + tid * 16) = now;
   }
 #pragma unroll
   for (int n = 0; n < P; ++n) {
-    const uint32_t t = token(n);
     float q[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) q[i] = sc == sc ? scaled<INT8>(x[n][i], sc, inv) : 0.f;
-    if (t >= kept) *(uint32_t*)(base + t * D + d) = code4<INT8>(q[0], q[1], q[2], q[3]);
+    if (token(n) >= kept) *(uint32_t*)(base + token(n) * D + d) = code4<INT8>(q[0], q[1], q[2], q[3]);
   }
 }
 
@@ -538,13 +510,14 @@ namespace {
 template <typename T, bool INT8>
 void append_dim(const KvArgs& a, uint32_t head_dim, const void* k, uint32_t ldk, const void* v, uint32_t ldv,
                 const RopeArgs& p, hipStream_t s) {
-  const dim3 grid(a.rows / kKvPage + 2 * a.seqs, 2 * a.kv_heads);
+  const dim3 grid(a.rows / kKvBlock + 2 * a.seqs, 2 * a.kv_heads);
+  const size_t lds = p.inv_freq ? (size_t)4 * 4 * (p.rot / 2) * 2 * sizeof(double) : 0;
   if (head_dim == 64)
-    hipLaunchKernelGGL((kv8_append_kernel<T, 64, INT8>), grid, dim3(256), 0, s, a, k, ldk, v, ldv, p);
+    hipLaunchKernelGGL((kv8_append_kernel<T, 64, INT8>), grid, dim3(256), lds, s, a, k, ldk, v, ldv, p);
   else if (head_dim == 128)
-    hipLaunchKernelGGL((kv8_append_kernel<T, 128, INT8>), grid, dim3(256), 0, s, a, k, ldk, v, ldv, p);
+    hipLaunchKernelGGL((kv8_append_kernel<T, 128, INT8>), grid, dim3(256), lds, s, a, k, ldk, v, ldv, p);
   else
-    hipLaunchKernelGGL((kv8_append_kernel<T, 256, INT8>), grid, dim3(256), 0, s, a, k, ldk, v, ldv, p);
+    hipLaunchKernelGGL((kv8_append_kernel<T, 256, INT8>), grid, dim3(256), lds, s, a, k, ldk, v, ldv, p);
 }
 template <typename T>
 void append_format(const KvArgs& a, uint32_t head_dim, bool int8, const void* k, uint32_t ldk, const void* v,
