@@ -8,6 +8,7 @@
 //   copy    moves whole pages, 16 bytes a lane.
 //
 // All three are bound by memory: each value is read once and written once.
+#include <algorithm>
 #include <cmath>
 
 #include "kv8_device.h"
@@ -315,15 +316,17 @@ __device__ __forceinline__ float wave_amax(const float* x) {
 
 // A workgroup is one block (16 tokens of one head, K or V). K: a wave takes four tokens, 4 dims a lane. V: a thread takes
 // one dim of 16, 8 or 4 tokens (D = 256, 128, 64), which are consecutive bytes. The waves meet once, over the largest
-// magnitude. With a wave per block, and so four times fewer waves with four times the work each, 2,307 rows took 18.7 us
-// against XX.
+// magnitude. With a wave per block, and so four times fewer waves with four times the work each, 2,307 rows of 4 heads
+// of 256 took 18.7 us against 14.0, one row of each of 64 sequences 12.4 against 7.4.
 template <typename T, int D, bool INT8>
 __global__ __launch_bounds__(256) void kv8_append_kernel(KvArgs a, const void* __restrict__ k, uint32_t ldk,
-                                                         const void* __restrict__ v, uint32_t ldv, RopeArgs rope) {
+                                                         const void* __restrict__ v, uint32_t ldv, RopeArgs rope,
+                                                         uint32_t at_once) {
   extern __shared__ __attribute__((aligned(16))) double angles[];  // (cos, sin) [4 waves][4 tokens][rot / 2]
-  __shared__ float amax[4];
-  const uint32_t head = blockIdx.y % a.kv_heads;
-  const bool is_v = blockIdx.y >= a.kv_heads;
+  __shared__ float amax[2][4];
+  const uint32_t groups = (a.kv_heads + at_once - 1) / at_once;
+  const bool is_v = blockIdx.y >= groups;
+  const uint32_t head0 = blockIdx.y % groups * at_once, head1 = min(head0 + at_once, a.kv_heads);
   uint32_t r0, r1;
   const uint32_t s = kv_find_seq(a.row0, a.seqs, a.rows, blockIdx.x, 1, kKvBlock, 2, r0, r1);
   if (s >= a.seqs || r1 <= r0) return;
@@ -335,55 +338,64 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(KvArgs a, const void* _
   if (id >= a.pages) return;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, block = (uint32_t)(t0 % kKvPage) / kKvBlock;
   uint8_t* const rec = a.pool + id * a.page_bytes;
-  float* const scale = (float*)(rec + kv_scale_at<D>(head, a.kv_heads)) + (is_v ? 4 : 0) + block;
+  auto scale_of = [&](uint32_t head) {
+    return (float*)(rec + kv_scale_at<D>(head, a.kv_heads)) + (is_v ? 4 : 0) + block;
+  };
   const uint32_t kept = p0 > t0 ? (uint32_t)(p0 - t0) : 0;                    // earlier tokens of the block
   const uint32_t end = p1 < t0 + kKvBlock ? (uint32_t)(p1 - t0) : kKvBlock;  // its new tokens are kept .. end - 1
-  const float before = kept ? *scale : 0.f;
   const size_t row = r0 + (size_t)(t0 - p0);  // the row of the block's token 0 (wraps below zero before row r0)
   auto row_of = [&](uint32_t t) { return row + min(max(t, kept), end - 1); };  // one of the call's in place of others
 
   // the block's scale, once the waves have left what they say
-  auto block_scale_now = [&](float mine) {
-    if (lane == 0) amax[wave] = mine;
+  auto block_scale_now = [&](uint32_t head, float before, float mine) {
+    float* const said = amax[head % 2];  // what the head before left is read by now, not what this one's will
+    if (lane == 0) said[wave] = mine;
     __syncthreads();
-    const float a0 = amax[0], a1 = amax[1], a2 = amax[2], a3 = amax[3];
+    const float a0 = said[0], a1 = said[1], a2 = said[2], a3 = said[3];
     const float sum = a0 + a1 + a2 + a3;  // NaN where one is
     const float fresh = block_scale<INT8>(fmaxf(fmaxf(a0, a1), fmaxf(a2, a3)));
     const float sc = sum != sum || (kept && before != before) ? NAN : kept ? fmaxf(fresh, before) : fresh;
-    if (tid == 0) *scale = sc;
+    if (tid == 0) *scale_of(head) = sc;
     return sc;
   };
 
   if (is_v) {
     constexpr int N = kKvBlock * D / 256;  // tokens of a thread
     const uint32_t d = tid % D, tok = tid / D * N;
-    Raw<T, 1> raw[N];
-#pragma unroll
-    for (int t = 0; t < N; ++t) raw[t].load(v, row_of(tok + t) * ldv + head * D + d);
     struct alignas(N) Words {
       uint32_t w[N / 4];
     };
-    Words* const at = (Words*)(rec + kv_v_at<D>(head, a.kv_heads) + (size_t)d * kKvPage + block * kKvBlock + tok);
-    Words old{};
-    if (kept) old = *at;
-    float x[N];
+    Raw<T, 1> raw[N];
+    auto load = [&](uint32_t head) {
 #pragma unroll
-    for (int t = 0; t < N; ++t) x[t] = tok + t >= kept && tok + t < end ? raw[t][0] : 0.f;
-    const float sc = block_scale_now(wave_amax<N>(x));
-    const float inv = 1.0f / sc, ratio = before / sc;
-    Words out;
+      for (int t = 0; t < N; ++t) raw[t].load(v, row_of(tok + t) * ldv + head * D + d);
+    };
+    load(head0);
+    for (uint32_t head = head0; head < head1; ++head) {
+      Words* const at = (Words*)(rec + kv_v_at<D>(head, a.kv_heads) + (size_t)d * kKvPage + block * kKvBlock + tok);
+      Words old{};
+      float before = 0.f;
+      if (kept) old = *at, before = *scale_of(head);
+      float x[N];
 #pragma unroll
-    for (int w = 0; w < N / 4; ++w) {
-      float q[4];
+      for (int t = 0; t < N; ++t) x[t] = tok + t >= kept && tok + t < end ? raw[t][0] : 0.f;
+      load(min(head + 1, head1 - 1));
+      const float sc = block_scale_now(head, before, wave_amax<N>(x));
+      const float inv = 1.0f / sc, ratio = before / sc;
+      Words out;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) q[i] = sc == sc ? scaled<INT8>(x[4 * w + i], sc, inv) : 0.f;
-      const int stay = (int)kept - (int)tok - 4 * w;  // bytes of tokens that stay
-      const uint32_t m = stay >= 4 ? ~0u : stay <= 0 ? 0u : (1u << 8 * stay) - 1u;
-      uint32_t o = old.w[w];
-      if (kept && sc > before) o = recode4<INT8>(o, ratio);
-      out.w[w] = (o & m) | (code4<INT8>(q[0], q[1], q[2], q[3]) & ~m);
+      for (int w = 0; w < N / 4; ++w) {
+        float q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = sc == sc ? scaled<INT8>(x[4 * w + i], sc, inv) : 0.f;
+        const int stay = (int)kept - (int)tok - 4 * w;  // bytes of tokens that stay
+        const uint32_t m = stay >= 4 ? ~0u : stay <= 0 ? 0u : (1u << 8 * stay) - 1u;
+        uint32_t o = old.w[w];
+        if (kept && sc > before) o = recode4<INT8>(o, ratio);
+        out.w[w] = (o & m) | (code4<INT8>(q[0], q[1], q[2], q[3]) & ~m);
+      }
+      *at = out;
     }
-    *at = out;
     return;
   }
 
@@ -393,23 +405,17 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(KvArgs a, const void* _
   const uint32_t d = 4 * (lane % W);
   auto token = [&](int n) { return 4 * wave + n * TP + lane / W; };
   Raw<T, 4> raw[P];
+  auto load = [&](uint32_t head) {
 #pragma unroll
-  for (int n = 0; n < P; ++n) raw[n].load(k, row_of(token(n)) * ldk + head * D + d);
-  // the block as it was, 16 bytes a thread
-  uint8_t* const base = rec + kv_k_at<D>(head) + (size_t)block * kKvBlock * D;
-  u4 old = u4{0, 0, 0, 0};
-  const bool stays = tid * 16 / D < kept;  // (a thread's 16 bytes are one token's)
-  if (stays) old = *(const u4*)(base + tid * 16);
-  float x[P][4];
-#pragma unroll
-  for (int n = 0; n < P; ++n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[n][i] = raw[n][i];
-  if (rope.inv_freq && 4 * wave < end && 4 * wave + 4 > kept) {
-    Turn<double> turn;
+    for (int n = 0; n < P; ++n) raw[n].load(k, row_of(token(n)) * ldk + head * D + d);
+  };
+  load(head0);
+  const bool turning = rope.inv_freq && 4 * wave < end && 4 * wave + 4 > kept;
+  const uint32_t pairs = rope.rot / 2;
+  double(*const cs)[2] = (double(*)[2])angles + (size_t)wave * 4 * pairs;
+  Turn<double> turn;
+  if (turning) {
     turn.init(rope, lane % W, D, rope.add_one ? 1.0 : 0.0);
-    const uint32_t pairs = rope.rot / 2;
-    double(*const cs)[2] = (double(*)[2])angles + (size_t)wave * 4 * pairs;
     for (uint32_t i = lane; i < 4 * pairs; i += 64) {
       const uint32_t pair = i % pairs, t = 4 * wave + i / pairs;
       if (t < kept || t >= end) continue;
@@ -420,35 +426,51 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(KvArgs a, const void* _
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // this wave's own reads follow
     __builtin_amdgcn_wave_barrier();
+  }
+  const bool stays = tid * 16 / D < kept;  // the thread's 16 bytes of the block as it was, which are one token's
+  for (uint32_t head = head0; head < head1; ++head) {
+    uint8_t* const base = rec + kv_k_at<D>(head) + (size_t)block * kKvBlock * D;
+    u4 old = u4{0, 0, 0, 0};
+    float before = 0.f;
+    if (stays) old = *(const u4*)(base + tid * 16);
+    if (kept) before = *scale_of(head);
+    float x[P][4];
+#pragma unroll
+    for (int n = 0; n < P; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[n][i] = raw[n][i];
+    load(min(head + 1, head1 - 1));
+    if (turning) {
+#pragma unroll
+      for (int n = 0; n < P; ++n) {
+        if (4 * wave + n * TP >= end || 4 * wave + n * TP + TP <= kept) continue;
+        const double inv = rope.norm_w ? norm_factor<W, double>(x[n], D, rope.eps) : 1.0;
+        double y[4];
+        turn4<T, W, double>(x[n], k, row_of(token(n)) * ldk + head * D, rope, turn, inv, cs + token(n) % 4 * pairs, y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[n][i] = (float)y[i];
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < P; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[n][i] = token(n) >= kept && token(n) < end ? x[n][i] : 0.f;
+    const float sc = block_scale_now(head, before, wave_amax<P * 4>(&x[0][0]));
+    const float inv = 1.0f / sc;
+    if (stays && sc > before) {
+      const float ratio = before / sc;
+      u4 now;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) now[w] = recode4<INT8>(old[w], ratio);
+      *(u4*)(base + tid * 16) = now;
+    }
 #pragma unroll
     for (int n = 0; n < P; ++n) {
-      if (4 * wave + n * TP >= end || 4 * wave + n * TP + TP <= kept) continue;
-      const double inv = rope.norm_w ? norm_factor<W, double>(x[n], D, rope.eps) : 1.0;
-      double y[4];
-      turn4<T, W, double>(x[n], k, row_of(token(n)) * ldk + head * D, rope, turn, inv, cs + token(n) % 4 * pairs, y);
+      float q[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[n][i] = (float)y[i];
+      for (int i = 0; i < 4; ++i) q[i] = sc == sc ? scaled<INT8>(x[n][i], sc, inv) : 0.f;
+      if (token(n) >= kept) *(uint32_t*)(base + token(n) * D + d) = code4<INT8>(q[0], q[1], q[2], q[3]);
     }
-  }
-#pragma unroll
-  for (int n = 0; n < P; ++n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[n][i] = token(n) >= kept && token(n) < end ? x[n][i] : 0.f;
-  const float sc = block_scale_now(wave_amax<P * 4>(&x[0][0]));
-  const float inv = 1.0f / sc;
-  if (stays && sc > before) {
-    const float ratio = before / sc;
-    u4 now;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) now[w] = recode4<INT8>(old[w], ratio);
-    *(u4*)(base + tid * 16) = now;
-  }
-#pragma unroll
-  for (int n = 0; n < P; ++n) {
-    float q[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = sc == sc ? scaled<INT8>(x[n][i], sc, inv) : 0.f;
-    if (token(n) >= kept) *(uint32_t*)(base + token(n) * D + d) = code4<INT8>(q[0], q[1], q[2], q[3]);
   }
 }
 
@@ -510,14 +532,22 @@ namespace {
 template <typename T, bool INT8>
 void append_dim(const KvArgs& a, uint32_t head_dim, const void* k, uint32_t ldk, const void* v, uint32_t ldv,
                 const RopeArgs& p, hipStream_t s) {
-  const dim3 grid(a.rows / kKvBlock + 2 * a.seqs, 2 * a.kv_heads);
+  // A workgroup takes one head after another where there would be more of them than run at once (four a CU):
+  // 385 blocks of 8 heads 21.4 us with one head each, 17.0 with four, 15.9 with eight; 146 blocks of 4 heads 14.0 with one,
+  // 15.9 with two.
+  const uint64_t single = ((uint64_t)a.rows / kKvBlock + a.seqs) * 2 * a.kv_heads;
+  const uint32_t at_once = (uint32_t)std::min<uint64_t>(a.kv_heads, std::max<uint64_t>(1, single / 1024));
+  const dim3 grid(a.rows / kKvBlock + 2 * a.seqs, 2 * ((a.kv_heads + at_once - 1) / at_once));
   const size_t lds = p.inv_freq ? (size_t)4 * 4 * (p.rot / 2) * 2 * sizeof(double) : 0;
   if (head_dim == 64)
-    hipLaunchKernelGGL((kv8_append_kernel<T, 64, INT8>), grid, dim3(256), lds, s, a, k, ldk, v, ldv, p);
+    hipLaunchKernelGGL((kv8_append_kernel<T, 64, INT8>), grid, dim3(256), lds, s, a, k, ldk, v, ldv, p,
+                       at_once);
   else if (head_dim == 128)
-    hipLaunchKernelGGL((kv8_append_kernel<T, 128, INT8>), grid, dim3(256), lds, s, a, k, ldk, v, ldv, p);
+    hipLaunchKernelGGL((kv8_append_kernel<T, 128, INT8>), grid, dim3(256), lds, s, a, k, ldk, v, ldv, p,
+                       at_once);
   else
-    hipLaunchKernelGGL((kv8_append_kernel<T, 256, INT8>), grid, dim3(256), lds, s, a, k, ldk, v, ldv, p);
+    hipLaunchKernelGGL((kv8_append_kernel<T, 256, INT8>), grid, dim3(256), lds, s, a, k, ldk, v, ldv, p,
+                       at_once);
 }
 template <typename T>
 void append_format(const KvArgs& a, uint32_t head_dim, bool int8, const void* k, uint32_t ldk, const void* v,
