@@ -220,11 +220,11 @@ int dh_kv8_attention_ws(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, ui
   if (rc != DH_OK) return rc;
   if (!ctx) return fail(DH_EINVAL, "kv8_attention_ws: null context");
   if (rows == 0 || seqs == 0) return ok();
-  const dh::KvAttnPlan plan = dh::kv8_attention_plan(rows, seqs, heads, cache->kv_heads, cache->head_dim,
-                                                     max_tokens / DH_KV8_PAGE + 1, max_tokens, ctx->cus);
+  const uint64_t bytes =
+      dh::kv8_attention_ws_bytes(rows, heads, cache->kv_heads, cache->head_dim, max_tokens, ctx->cus);
   float* aux = nullptr;
-  if (plan.ws_bytes) {
-    rc = ensure_aux(ctx, (hipStream_t)stream, plan.ws_bytes, &aux);
+  if (bytes) {
+    rc = ensure_aux(ctx, (hipStream_t)stream, bytes, &aux);
     if (rc != DH_OK) return rc;
   }
   return ok();

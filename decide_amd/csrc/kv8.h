@@ -55,6 +55,8 @@ struct KvAttnPlan {
 };
 KvAttnPlan kv8_attention_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
                               uint32_t ld_table, uint32_t max_tokens, uint32_t cus);
+uint64_t kv8_attention_ws_bytes(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_tokens,
+                                uint32_t cus);
 hipError_t launch_kv8_attention(const KvArgs& a, uint32_t head_dim, bool int8, const _Float16* q, uint32_t ldq,
                                 uint32_t heads, float scale, const float* gate, uint32_t ldg, _Float16* y,
                                 uint32_t ldy, float* ws, const KvAttnPlan& plan, hipStream_t s);

@@ -212,23 +212,26 @@ __device__ __forceinline__ uint32_t tile_at(const Deal<SLOTS>& d, uint32_t slots
   return lo;
 }
 
-// Four outputs of row r: O times `factor`, times the gate's sigmoid.
-template <bool GATE>
-__device__ __forceinline__ void store_out(const AttnArgs& t, uint32_t r, uint32_t col, const f4& acc, float factor) {
+// Four outputs of row r: O times `factor`, times the sigmoid of the gate where there is one.
+__device__ __forceinline__ void store_out(const AttnArgs& t, uint32_t r, uint32_t col, const f4& acc, float factor,
+                                          const f4& gate) {
   f4 v = acc * factor;
-  if constexpr (GATE) {
-    const f4 gt = *(const f4*)(t.gate + (size_t)r * t.ldg + col);
+  if (t.gate) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] *= sigmoid(gt[e]);
+    for (int e = 0; e < 4; ++e) v[e] *= sigmoid(gate[e]);
   }
   *(h4*)(t.y + (size_t)r * t.ldy + col) = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
 }
-
-__device__ __forceinline__ void store_out(const AttnArgs& t, uint32_t r, uint32_t col, const f4& acc, float factor) {
-  if (t.gate)
-    store_out<true>(t, r, col, acc, factor);
-  else
-    store_out<false>(t, r, col, acc, factor);
+// eight dims, already over their sum
+__device__ __forceinline__ void store_out8(const AttnArgs& t, uint32_t r, uint32_t col, f4 v0, f4 v1, const f4& g0,
+                                           const f4& g1) {
+  typedef _Float16 h8u __attribute__((ext_vector_type(8), aligned(8)));
+  if (t.gate) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v0[e] *= sigmoid(g0[e]), v1[e] *= sigmoid(g1[e]);
+  }
+  *(h8u*)(t.y + (size_t)r * t.ldy + col) = h8u{(_Float16)v0[0], (_Float16)v0[1], (_Float16)v0[2], (_Float16)v0[3],
+                                               (_Float16)v1[0], (_Float16)v1[1], (_Float16)v1[2], (_Float16)v1[3]};
 }
 __device__ __forceinline__ float over_sum(float l) { return l == 0.f ? 0.f : 1.0f / l; }  // a row that sees nothing is 0
 

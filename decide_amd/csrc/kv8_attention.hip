@@ -17,9 +17,8 @@
 //     kv head (one per CU in all) add up the pages of all tiles, each for itself, and take equal runs of them: a run may
 //     end one tile and begin another. A tile that lies in several runs leaves a state (largest score, sum, O) per run, and
 //     kv8_combine_kernel merges them in order. With pieces of a fixed length instead, sized by the longest sequence, 64
-//     sequences of up to 8,192 tokens made 2,560 workgroups, 2,100 of them empty, and took 77 us against XX.
+//     sequences of up to 8,192 tokens made 2,560 workgroups, 2,100 of them empty, and took 77 us against 52.
 #include <algorithm>
-#include <cstdlib>
 
 #include "kv8_attention.h"
 
@@ -80,6 +79,14 @@ __global__ __launch_bounds__(512) void kv8_attention_kernel(KvArgs a, AttnArgs t
         for (int j = 0; j < 2 * S; ++j) q[j] = -q[j];
       }
     }
+    // the gate of the thread's first four outputs, in flight through the pages
+    const uint32_t pairs = min(kKvTile, tile.pairs);
+    f4 gate = f4{0.f, 0.f, 0.f, 0.f};
+    if (t.gate && whole && tid < pairs * (D / 4)) {
+      uint32_t r, h;
+      pair_at(t, tile, kvh, tid / (D / 4), r, h);
+      gate = *(const f4*)(t.gate + (size_t)r * t.ldg + h * D + 4 * (tid % (D / 4)));
+    }
     f4 o[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
@@ -127,9 +134,10 @@ __global__ __launch_bounds__(512) void kv8_attention_kernel(KvArgs a, AttnArgs t
         for (int i = 0; i < 16; ++i) sv[i] = i < (int)mine ? sv[i] * cs : -INFINITY;
         unit = 1.0f;
         blind = mine == 0;
-        if (tok0 >= most) vs = 0.f;  // the scale of a block that none sees may be anything
-        if (b * kKvPage + (kKvPage - 1) >= most) {  // bytes behind the last seen token may be anything
-          const uint32_t have = most > tok0 ? min(most - tok0, 16u) : 0;
+        // What none sees may be anything, and so may what stands in for a bad page, for those that do not see it.
+        if (tok0 >= most || bad) vs = 0.f;
+        if (b * kKvPage + (kKvPage - 1) >= most || bad) {
+          const uint32_t have = most > tok0 && !bad ? min(most - tok0, 16u) : 0;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             const int left = (int)have - 4 * w;
@@ -173,7 +181,6 @@ __global__ __launch_bounds__(512) void kv8_attention_kernel(KvArgs a, AttnArgs t
     }
 
     // The waves meet: each leaves its O relative to the largest of their reference points.
-    const uint32_t pairs = min(kKvTile, tile.pairs);
     l = sum_groups(l);
     if (g == 0) ml[wave * kKvTile + n] = f2{m, l};
     __syncthreads();
@@ -202,7 +209,8 @@ __global__ __launch_bounds__(512) void kv8_attention_kernel(KvArgs a, AttnArgs t
       if (whole) {
         uint32_t r, h;
         pair_at(t, tile, kvh, pr, r, h);
-        store_out(t, r, h * D + d, acc, over_sum(lt));
+        if (t.gate && i != tid) gate = *(const f4*)(t.gate + (size_t)r * t.ldg + h * D + d);
+        store_out(t, r, h * D + d, acc, over_sum(lt), gate);
       } else {
         *(f4*)(state + pr * D + d) = acc;
         if (d == 0) *(f2*)(state + kKvTile * D + 2 * pr) = f2{top, lt};
@@ -215,84 +223,114 @@ __global__ __launch_bounds__(512) void kv8_attention_kernel(KvArgs a, AttnArgs t
 }
 
 // Merges the states of every tile that lies in more than one run, in the runs' order, and writes the rows that see
-// nothing. A workgroup per tile, kv head and 16 pairs of it: D / 4 lanes a pair, and where the pairs leave lanes over,
-// several groups take every so many runs of a pair.
-template <int D, uint32_t TILE>
+// nothing. A workgroup takes PAIRS pairs of a tile, D / 4 lanes a pair, and the 512 / (PAIRS D / 4) groups of lanes that a
+// pair has take every so many of its states, merged as they come: each state is one read behind the others', whatever
+// their number.
+template <int D, uint32_t TILE, uint32_t PAIRS>
 __global__ __launch_bounds__(512) void kv8_combine_kernel(KvArgs a, AttnArgs t) {
-  constexpr uint32_t L = D / 4, kParts = TILE / 16;
-  __shared__ __attribute__((aligned(16))) f4 sum[512];
-  __shared__ float lsum[512];
+  constexpr uint32_t L = D / 4, kParts = TILE / PAIRS, kItems = PAIRS * L, kWays = 512 / kItems;
+  static_assert(kItems * kWays == 512 && TILE % PAIRS == 0, "a pair's lanes and ways fill the workgroup");
+  __shared__ __attribute__((aligned(16))) f4 sums[512];
+  __shared__ f2 mls[512];
   const uint32_t kvh = blockIdx.x % a.kv_heads, part = blockIdx.x / a.kv_heads % kParts,
                  slot = blockIdx.x / a.kv_heads / kParts, tid = threadIdx.x;
   const uint32_t* const before = starts_of<D, TILE>(a, t);
-  const uint32_t u0 = before[slot], u1 = before[slot + 1], share = share_of(before[t.slots], t);
+  const uint32_t u0 = before[slot], u1 = before[slot + 1], total = before[t.slots];
+  Tile tile;
+  if (!find_tile<TILE>(a, t.group, slot, tile) || PAIRS * part >= tile.pairs) return;
+  const uint32_t share = share_of(total, t);
   const uint32_t w0 = u0 / share, w1 = u1 > u0 ? (u1 - 1) / share : w0;
   if (u1 > u0 && w0 == w1) return;  // written by the attention kernel itself
-  Tile tile;
-  if (!find_tile<TILE>(a, t.group, slot, tile) || 16 * part >= tile.pairs) return;
-  const uint32_t pairs = min(16u, tile.pairs - 16 * part);
-  const uint32_t items = pairs * L;
-  // `ways` groups of `items` lanes, or several rounds of one group
-  const uint32_t ways = items <= 256 ? 512 / items : 1;
-  const uint32_t way = ways > 1 ? tid / items : 0;
-  for (uint32_t i0 = 0; i0 < items; i0 += 512) {
-    const uint32_t i = ways > 1 ? tid % items : i0 + tid;
-    const uint32_t pr = 16 * part + i / L, d = 4 * (i % L);
-    const bool on = i < items && way < ways;
-    f4 acc = f4{0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    if (on && u1 > u0) {
-      auto state = [&](uint32_t w) { return state_of<D, TILE>(t, kvh, w, w == w0 && u0 != w0 * share ? 1 : 0); };
-      float top = -INFINITY;
-#pragma unroll 8
-      for (uint32_t w = w0; w <= w1; ++w) top = fmaxf(top, state(w)[TILE * D + 2 * pr]);
+  const uint32_t item = tid % kItems, way = tid / kItems, d = 4 * (item % L);
+  const uint32_t pr = min(PAIRS * part + item / L, tile.pairs - 1);
+  f4 acc = f4{0.f, 0.f, 0.f, 0.f};
+  float top = -INFINITY, l = 0.f;
+  if (u1 > u0) {
 #pragma unroll 4
-      for (uint32_t w = w0 + way; w <= w1; w += ways) {
-        const float* const s = state(w);
-        const f2 v = *(const f2*)(s + TILE * D + 2 * pr);
-        const float x = state_weight(v[0], top);
-        l += v[0] == -INFINITY ? v[1] : v[1] * x;
-        acc += *(const f4*)(s + pr * D + d) * x;
-      }
-    }
-    if (ways > 1) {
-      sum[tid] = acc;
-      lsum[tid] = l;
-      __syncthreads();
-      if (way == 0)
-        for (uint32_t j = 1; j < ways; ++j) {
-          acc += sum[j * items + i];
-          l += lsum[j * items + i];
-        }
-    }
-    if (on && way == 0) {
-      uint32_t r, h;
-      pair_at(t, tile, kvh, pr, r, h);
-      store_out(t, r, h * D + d, acc, over_sum(l));
+    for (uint32_t w = w0 + way; w <= w1; w += kWays) {
+      const float* const s = state_of<D, TILE>(t, kvh, w, w == w0 && u0 != w0 * share ? 1 : 0);
+      const f2 v = *(const f2*)(s + TILE * D + 2 * pr);
+      const f4 o = *(const f4*)(s + pr * D + d);
+      const float both = fmaxf(top, v[0]), x = state_weight(top, both), y = state_weight(v[0], both);
+      l = (top == -INFINITY ? l : l * x) + (v[0] == -INFINITY ? v[1] : v[1] * y);  // a NaN sum stays
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(o[e], y, acc[e] * x);
+      top = both;
     }
   }
+  if constexpr (kWays > 1) {
+    sums[tid] = acc;
+    mls[tid] = f2{top, l};
+    __syncthreads();
+    if (way != 0) return;
+#pragma unroll
+    for (uint32_t j = 1; j < kWays; ++j) {
+      const f2 v = mls[j * kItems + item];
+      const f4 o = sums[j * kItems + item];
+      const float both = fmaxf(top, v[0]), x = state_weight(top, both), y = state_weight(v[0], both);
+      l = (top == -INFINITY ? l : l * x) + (v[0] == -INFINITY ? v[1] : v[1] * y);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(o[e], y, acc[e] * x);
+      top = both;
+    }
+  }
+  if (PAIRS * part + item / L >= tile.pairs) return;
+  uint32_t r, h;
+  pair_at(t, tile, kvh, pr, r, h);
+  f4 gate = f4{0.f, 0.f, 0.f, 0.f};
+  if (t.gate) gate = *(const f4*)(t.gate + (size_t)r * t.ldg + h * D + d);
+  store_out(t, r, h * D + d, acc, over_sum(l), gate);
 }
+
+namespace {
+uint64_t least_pages(bool wide, uint32_t head_dim) {
+  return wide ? 64 : head_dim == 256 ? 17 : head_dim == 128 ? 25 : 57;
+}
+
+// Two states for each run, and where each slot's runs start.
+uint64_t run_bytes(bool wide, uint64_t runs, uint64_t slots, uint32_t kv_heads, uint32_t head_dim) {
+  return (kv_heads * runs * 2 * ((wide ? kKvWideTile : kKvTile) * (head_dim + 2)) + slots + 1) * sizeof(float);
+}
+}  // namespace
 
 KvAttnPlan kv8_attention_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
                               uint32_t ld_table, uint32_t max_tokens, uint32_t cus) {
   KvAttnPlan p;
   const uint64_t pairs = (uint64_t)rows * (heads / kv_heads);
-  p.wide = pairs >= 64ull * seqs;
-  static const char* force = getenv("KV8_WIDE");
-  if (force) p.wide = atoi(force);
+  const uint64_t pages = std::min<uint64_t>(((uint64_t)max_tokens + kKvPage - 1) / kKvPage, ld_table);
+  const uint64_t full = pairs / kKvTile * kv_heads;  // narrow tiles that are surely full
+  // Many rows: tiles of 128 pairs. 16 heads over 4 of 256: 496 causal rows 33 us against 25 with tiles of 16, 603 rows 32
+  // against 32, 1,000 rows 44 against 54, 8 x 128 rows 46 against 70; 32 over 8 of 128: 256 rows behind 544 tokens 25
+  // against 18, 496 rows 22 against 26. Heads of 64 dims leave the narrow kernel room for two workgroups a CU: 8 heads over
+  // one, 1,500 causal rows 30 against 14, 4,000 rows 69 against 54, 8,000 rows 141 against 155, 16 x 512 rows behind 2,000
+  // tokens 61 against 84. Few rows behind many tokens, where the narrow kernel reads them once for every 16 pairs: 256 rows
+  // of 4 heads behind 7,744 tokens 72 against 91, 128 rows behind 3,972 tokens 48 against 44.
+  p.wide = head_dim == 64 ? full >= 10ull * cus
+                          : full >= 5ull * cus / 2 || (pages >= least_pages(true, head_dim) && pairs >= 512ull * seqs);
   const uint32_t tile = p.wide ? kKvWideTile : kKvTile;
   const uint64_t slots = pairs / tile + seqs;
   p.slots = (uint32_t)slots;
-  const uint64_t pages = std::min<uint64_t>(((uint64_t)max_tokens + kKvPage - 1) / kKvPage, ld_table);
-  if (pages <= (p.wide ? 4 : 16) || slots > (p.wide ? kKvWideSlots : kKvMaxSlots) || slots * (ld_table + 1ull) > UINT32_MAX) return p;
-  static const char* fr = getenv("KV8_RUNS");
-  const int mul = fr ? atoi(fr) : p.wide && slots * kv_heads >= cus ? 0 : 1;
-  if (mul == 0) return p;
-  p.runs = std::max<uint32_t>(1, mul * cus / kv_heads);
-  static const char* fm = getenv("KV8_MIN");
-  p.min_run = p.wide ? (fm ? atoi(fm) : 4) : 8;
-  p.ws_bytes = ((uint64_t)kv_heads * p.runs * 2 * (tile * (head_dim + 2)) + kKvMaxSlots + 1) * sizeof(float);
+  // Runs, where whole tiles would leave most CUs idle behind long sequences, at the price of the count of their pages and
+  // of the merge. One row, 16 heads over 4 of 256: 1,100 tokens 15.0 us against 17.1 with a workgroup per tile, 8,000
+  // tokens 16 against 87; heads of 128: 1,100 tokens 11.9 against 10.3, 2,000 12.1 against 15.6; heads of 64: 3,000
+  // tokens 10.6 against 10.2, 8,000 11.1 against 19.8. 1,500 rows in runs: 341 against 95. Wide tiles of 4 heads of 256:
+  // 256 rows behind 7,744 tokens 72 against 212, 1,000 rows of 8,000 169 against 214, 1,000 causal rows 95 against 45.
+  if (pages < least_pages(p.wide, head_dim) || (p.wide ? slots * kv_heads : full) >= cus ||
+      (p.wide && head_dim == 64) || slots > (p.wide ? kKvWideSlots : kKvMaxSlots) || slots * (ld_table + 1ull) > UINT32_MAX)
+    return p;
+  p.runs = std::max<uint32_t>(1, cus / kv_heads);
+  p.min_run = p.wide ? 4 : 8;  // a page for each wave; fewer, and the states' share grows
+  p.ws_bytes = run_bytes(p.wide, p.runs, p.slots, kv_heads, head_dim);
   return p;
+}
+
+// What any call of at most these sizes takes.
+uint64_t kv8_attention_ws_bytes(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_tokens,
+                                uint32_t cus) {
+  const uint64_t pages = ((uint64_t)max_tokens + kKvPage - 1) / kKvPage;
+  if (pages < least_pages(false, head_dim)) return 0;
+  const bool wide = head_dim != 64 && pages >= least_pages(true, head_dim) && (uint64_t)rows * (heads / kv_heads) >= 512;
+  return run_bytes(wide, std::max<uint32_t>(1, cus / kv_heads), kKvMaxSlots, kv_heads, head_dim);
 }
 
 namespace {
@@ -311,11 +349,17 @@ hipError_t attention_of(const KvArgs& a, const AttnArgs& t, bool int8, bool wide
   if (!wide) narrow_kernels<D>(a, t, int8, s);
   const hipError_t e = wide ? launch_kv8_wide(a, t, D, int8, s) : hipGetLastError();
   if (!t.runs || e != hipSuccess) return e;
-  if (wide)
-    hipLaunchKernelGGL((kv8_combine_kernel<D, kKvWideTile>), dim3(a.kv_heads * t.slots * (kKvWideTile / 16)), dim3(512),
-                       0, s, a, t);
+  constexpr uint32_t kPairs = 512 / D;  // of a workgroup of the combine: four ways a pair
+  if (wide) {
+    if constexpr (D != 64)
+      hipLaunchKernelGGL((kv8_combine_kernel<D, kKvWideTile, kPairs>),
+                         dim3(a.kv_heads * t.slots * (kKvWideTile / kPairs)), dim3(512), 0, s, a, t);
+  } else if (a.kv_heads * t.slots * (kKvTile / kPairs) <= 1024)  // (four workgroups a CU)
+    hipLaunchKernelGGL((kv8_combine_kernel<D, kKvTile, kPairs>), dim3(a.kv_heads * t.slots * (kKvTile / kPairs)),
+                       dim3(512), 0, s, a, t);
   else
-    hipLaunchKernelGGL((kv8_combine_kernel<D, kKvTile>), dim3(a.kv_heads * t.slots), dim3(512), 0, s, a, t);
+    hipLaunchKernelGGL((kv8_combine_kernel<D, kKvTile, 2 * kPairs>), dim3(a.kv_heads * t.slots * (kKvTile / (2 * kPairs))),
+                       dim3(512), 0, s, a, t);
   return hipGetLastError();
 }
 }  // namespace
@@ -324,7 +368,7 @@ hipError_t launch_kv8_attention(const KvArgs& a, uint32_t head_dim, bool int8, c
                                 uint32_t heads, float scale, const float* gate, uint32_t ldg, _Float16* y,
                                 uint32_t ldy, float* ws, const KvAttnPlan& p, hipStream_t s) {
   if (a.rows == 0 || a.seqs == 0) return hipSuccess;
-  if (p.runs && (!ws || p.min_run == 0 || p.slots > (p.wide ? kKvWideSlots : kKvMaxSlots))) return hipErrorInvalidValue;
+  if (p.runs && (!ws || p.min_run == 0 || (p.wide && head_dim == 64) || p.slots > (p.wide ? kKvWideSlots : kKvMaxSlots))) return hipErrorInvalidValue;
   const uint32_t group = heads / a.kv_heads;
   const AttnArgs t{q,     gate,    y,      ws,        ldq,  ldg, ldy, heads, group, ((1u << 21) + group - 1) / group,
                    p.slots, p.runs, p.min_run, scale};

@@ -2,15 +2,16 @@
 //
 // kv8_attention_wide_kernel, tiles of 128 (row, head) pairs: eight waves, four groups of 32 pairs x the two halves of a
 // page's blocks, on v_mfma_f32_32x32x16_f16.
-//   * Pages go into LDS as they are, by DMA, two at a time into one of two buffers, one barrier per two pages; a wave
-//     reads the codes of its half from there and turns them into fp16 in registers, 128 conversions and 32 products of
-//     32 clocks a page.
+//   * Pages go into LDS as they are, by DMA, into a ring of four; a wave reads the codes of its half from there and turns
+//     them into fp16 in registers, 128 conversions and 32 products of 32 clocks a page.
 //   * The same deal of tokens as in kv8_attention_kernel, for two lane groups: lane (r, f), r = lane % 32, f = lane / 32,
 //     of half T gets the 16 scores of pair r and block 2 T + f, which are P^T V's operand as they are.
 //   * 16-byte chunk x of K's token t lies at chunk x ^ key(t), of V's dim d at x ^ (d / 2 % 4), so that eight lanes
 //     that read at once read 128 different bytes' banks.
-//   * Two waves of a SIMD share its issue port: alone, a wave issues an instruction of the vector unit every 6 to 7 clocks,
-//     two together one every 4. With four waves a workgroup, both halves a wave, 37 pages took 96 us against XX.
+//   * Bound by the issue of vector instructions: two waves of a SIMD have 340 each a page, 4 clocks apart at best (one wave
+//     alone issues every 6 to 7), and the matrix cores are busy for 2,048 clocks of a page's 4,100. The halves are kept half a
+//     page apart, and the one at its products has priority. With four waves, each taking both halves, 37 pages took 96 us
+//     against 76; with one barrier for all every two pages 82.
 //   * The two halves meet once, at a tile's end, through LDS: each takes half of the dims.
 #include "kv8_attention.h"
 
@@ -164,9 +165,10 @@ __global__ __launch_bounds__(512) void kv8_attention_wide_kernel(KvArgs a, AttnA
     for (uint32_t b = b0; b < b1; ++b) {
       const uint32_t at = (b - b0) & 3;
       if (T == 0) {
-        if (b * kKvPage + (kKvPage - 1) >= most) {  // bytes behind the last seen token may be anything
+        // Bytes behind the last seen token may be anything, and what stands in for a bad page too.
+        if (b * kKvPage + (kKvPage - 1) >= most || id0 >= a.pages) {
           char* const vb = lds + (at * 2 + 1) * kBytes;
-          const uint32_t have = most % kKvPage;
+          const uint32_t have = id0 >= a.pages ? 0 : most % kKvPage;
           for (uint32_t i = thread(); i < D * 4; i += 256) {
             const uint32_t dim = i / 4, x = i % 4, left = have > 16 * x ? min(have - 16 * x, 16u) : 0;
             u4* const to = (u4*)(vb + dim * 64 + (x ^ (dim >> 1 & 3)) * 16);
@@ -221,7 +223,7 @@ __global__ __launch_bounds__(512) void kv8_attention_wide_kernel(KvArgs a, AttnA
           for (int i = 0; i < 16; ++i) st[i] = i < (int)mine ? st[i] * cs : -INFINITY;
           unit = 1.0f;
           blind = mine == 0;
-          if (tok0 >= most) vs = 0.f;
+          if (tok0 >= most || bad) vs = 0.f;
         }
         float bm = st[0];
 #pragma unroll
@@ -278,50 +280,72 @@ __global__ __launch_bounds__(512) void kv8_attention_wide_kernel(KvArgs a, AttnA
     __syncthreads();  // the states go where the pages lie
 
     // The halves' states meet: each wave keeps its first o's and gives its partner the rest.
+    constexpr uint32_t kPer = DT / 2 * 4;  // pieces of four dims that a lane keeps: dims D/2 T + 32 (i / 4) + 8 (i % 4) + 4 f
     const uint32_t lane = thread() & 63, r = lane & 31, f = lane >> 5;
     f4* const xo = (f4*)lds;
+    // piece i of lane x: the swizzle spreads one pair's pieces over the banks
+    auto piece = [](uint32_t of, uint32_t i, uint32_t x) { return (of * kPer + i) * 64 + (x ^ i); };
     l = sum_halves(l);
     if (f == 0) meet[wave * 32 + r] = f4{m, l, vref, 0.f};
 #pragma unroll
-    for (int i = 0; i < DT / 2 * 4; ++i) {
+    for (int i = 0; i < (int)kPer; ++i) {
       const f16v& v = o[DT / 2 + i / 4];
       const int e = 4 * (i % 4);
-      xo[(wave * (DT / 2 * 4) + i) * 64 + lane] = f4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+      xo[piece(wave, i, lane)] = f4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+    }
+    // What a lane writes in the end: dims D/2 T + 8 x .. + 7 of pairs first + 64 / kPer k.
+    const uint32_t x = lane % kPer, first = 32 * group + lane / kPer, d = T * (D / 2) + 8 * x;
+    auto read_gate = [&](uint32_t k, f4* to) {
+      pair_at(t, tile, kvh, min(first + 64 / kPer * k, tile.pairs - 1), row, head);
+      const f4* const g = (const f4*)(t.gate + (size_t)row * t.ldg + head * D + d);
+      to[0] = g[0];
+      to[1] = g[1];
+    };
+    f4 gate[RUNS ? 2 : kPer];
+    if (!RUNS && t.gate) {  // while the exchange runs (in runs they would spill)
+#pragma unroll
+      for (uint32_t k = 0; k < kPer / 2; ++k) read_gate(k, gate + 2 * k);
     }
     __syncthreads();
-    if (32 * group + r < tile.pairs) {
+    {
       const f4 other = meet[(wave ^ 4) * 32 + r];
       const float top = fmaxf(m, other[0]);
       const float wm = state_weight(m, top), wo = state_weight(other[0], top);
       // (a NaN sum stays: a state without a score has weight 0 and, but for NaN, the sum 0)
       const float lt = (m == -INFINITY ? l : l * wm) + (other[0] == -INFINITY ? other[1] : other[1] * wo);
-      const float fm = wm * vref, fo = wo * other[2];
-      auto merged = [&](int i) {
-        const f4 po = xo[((wave ^ 4) * (DT / 2 * 4) + i) * 64 + lane];
+      const float factor = whole ? over_sum(lt) : 1.0f;
+      const float fm = wm * vref * factor, fo = wo * other[2] * factor;
+#pragma unroll
+      for (int i = 0; i < (int)kPer; ++i) {
+        f4& to = xo[piece(wave ^ 4, i, lane)];  // (read by this lane only)
+        const f4 po = to;
         f4 v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = fmaf(po[e], fo, o[i / 4][4 * (i % 4) + e] * fm);
-        return v;
-      };
-      const uint32_t d0 = T * (D / 2) + 4 * f;  // dims d0 + 32 (i / 4) + 8 (i % 4) ..
-      if (whole) {
-        pair_at(t, tile, kvh, 32 * group + r, row, head);
-        const float factor = over_sum(lt);
-        auto store = [&](auto gate) {
-#pragma unroll
-          for (int i = 0; i < DT / 2 * 4; ++i)
-            store_out<decltype(gate)::value>(t, row, head * D + d0 + 32 * (i / 4) + 8 * (i % 4), merged(i), factor);
-        };
-        if (t.gate)
-          store(std::true_type{});
-        else
-          store(std::false_type{});
-      } else {
+        to = v;
+      }
+      if (!whole && T == 0 && f == 0 && 32 * group + r < tile.pairs) {
         float* const state = state_of<D, kKvWideTile>(t, kvh, run, u == first_u ? 0 : 1);
-        float* const to = state + (32 * group + r) * D + d0;
+        *(f2*)(state + kKvWideTile * D + 2 * (32 * group + r)) = f2{top, lt};
+      }
+    }
+    // From LDS once more, now eight dims a lane and a pair's half in kPer lanes: gates, results and states in whole lines.
+    // Straight from the products' layout, 32 bytes of a line at a time, a tile's end took 11,000 to 29,000 clocks.
+    asm volatile("" ::: "memory");  // the wave's own writes, read by its other lanes: LDS keeps a wave's order
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < DT / 2 * 4; ++i) *(f4*)(to + 32 * (i / 4) + 8 * (i % 4)) = merged(i);
-        if (T == 0 && f == 0) *(f2*)(state + kKvWideTile * D + 2 * (32 * group + r)) = f2{top, lt};
+    for (uint32_t k = 0; k < kPer / 2; ++k) {
+      const uint32_t pair = first + 64 / kPer * k;
+      const f4 v0 = xo[piece(wave ^ 4, x, pair % 32)], v1 = xo[piece(wave ^ 4, x, pair % 32 + 32)];
+      if (pair >= tile.pairs) continue;
+      if (whole) {
+        if (RUNS && t.gate) read_gate(k, gate);
+        pair_at(t, tile, kvh, pair, row, head);
+        store_out8(t, row, head * D + d, v0, v1, gate[RUNS ? 0 : 2 * k], gate[RUNS ? 1 : 2 * k + 1]);
+      } else {
+        float* const to = state_of<D, kKvWideTile>(t, kvh, run, u == first_u ? 0 : 1) + pair * D + d;
+        *(f4*)to = v0;
+        *(f4*)(to + 4) = v1;
       }
     }
     if constexpr (!RUNS) return;
@@ -338,7 +362,12 @@ void wide_kernels(const KvArgs& a, const AttnArgs& t, bool int8, hipStream_t s) 
     hipLaunchKernelGGL((kv8_attention_wide_kernel<D, decltype(i8)::value, decltype(runs)::value>), grid, dim3(512), 0, s,
                        a, t);
   };
-  auto with = [&](auto i8) { t.runs ? go(i8, std::true_type{}) : go(i8, std::false_type{}); };
+  auto with = [&](auto i8) {
+    if constexpr (D != 64) {
+      if (t.runs) return go(i8, std::true_type{});
+    }
+    go(i8, std::false_type{});
+  };
   int8 ? with(std::true_type{}) : with(std::false_type{});
 }
 }  // namespace

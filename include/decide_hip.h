@@ -636,12 +636,16 @@ int dh_kv8_append(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, uint32_t
  * ldq % 8 == 0, ldy % 4 == 0, ldg % 4 == 0; q and gate 16-byte, y 8-byte
  * aligned. Long sequences are divided across workgroups and merged through the
  * context's forward-kernel workspace (dh_kv8_attention_ws; an eager call of
- * the same sizes also grows it): the cut depends on the call's sizes only. */
+ * the same sizes also grows it). The cuts depend on the call's sizes and on how
+ * many pages its rows see, found on the device: a row's bits depend on its own
+ * query, position and pages and, where its sequence is cut, on the other rows
+ * of the call (rounding only). The same call gives the same bits. */
 int dh_kv8_attention(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, uint32_t layer, const dh_kv8_batch* batch,
                      const uint16_t* q, uint32_t ldq, uint32_t heads, float scale, const float* gate, uint32_t ldg,
                      uint16_t* y, uint32_t ldy, uint32_t max_tokens);
 /* Grows `stream`'s forward-kernel workspace to what dh_kv8_attention needs for
- * these sizes (before a capture on that stream, for instance). */
+ * these sizes and any smaller ones (before a capture on that stream, for
+ * instance). */
 int dh_kv8_attention_ws(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, uint32_t rows, uint32_t seqs,
                         uint32_t heads, uint32_t max_tokens);
 

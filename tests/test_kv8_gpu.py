@@ -317,7 +317,9 @@ def run_attention(kernels, stream, t, heads, gate=True, scale=None, max_tokens=N
     return got[:, :wide].reshape(t.rows, heads, dim), got[:, wide:], q, g
 
 
-def check_attention(kernels, stream, t, heads, gate=True, scale=None, **kw):
+def check_attention(kernels, stream, t, heads, gate=True, scale=None, only=None, nan=None, **kw):
+    """`only`: the heads that are held to the reference (all of them, unless there are many rows). `nan`: rows and heads that
+    are NaN, left to the caller."""
     got, behind, q, g = run_attention(kernels, stream, t, heads, gate, scale, **kw)
     scale = t.dim ** -0.5 if scale is None else scale
     assert (behind == 7).all()
@@ -337,7 +339,9 @@ def check_attention(kernels, stream, t, heads, gate=True, scale=None, **kw):
             if m == 0:
                 assert (got[r] == 0).all()
                 continue
-            for h in range(heads):
+            for h in only or range(heads):
+                if nan is not None and nan[r, h]:
+                    continue
                 kh, vh = k[:m, h // group], v[:m, h // group]
                 sc = kh @ q[r, h] * scale
                 p = np.exp(sc - sc.max())
@@ -398,6 +402,65 @@ def test_attention_over_long_sequences(gpu, kernels, stream, fmt, heads, kv, dim
         assert np.allclose(again.astype(np.float64), got.astype(np.float64), rtol=2.0 ** -9, atol=2.0 ** -9)
 
 
+@pytest.mark.parametrize("gate", [True, False])
+@pytest.mark.parametrize("fmt,heads,kv,dim,rows", [
+    ("e4m3", 16, 4, 256, 520), ("int8", 32, 2, 256, 180), ("int8", 40, 8, 128, 120), ("e4m3", 96, 3, 128, 0),
+    ("e4m3", 72, 8, 64, 500), ("int8", 64, 4, 64, 560)])
+def test_attention_of_many_rows(gpu, kernels, stream, fmt, heads, kv, dim, rows, gate):
+    """Enough rows to fill the device with tiles of 128: ragged sequences of every kind, one of them `rows` rows, groups of
+    which 128 is no multiple among the layouts; a sequence that ends inside a page next to NaN codes and scales; NaN blocks
+    and a bad page that some rows see; rows that see nothing, in no order of positions."""
+    lens, counts = [rows + 70, 5, 333, 64, 9, 150, 1, 200], [rows, 0, 121, 64, 9, 1, 1, 60]
+    t = Setup(kv, dim, fmt, lens, counts, seed=dim + heads, layers=1, layer=0)
+    t.fill(lens)
+    r0, r1 = int(t.row0[2]), int(t.row0[3])
+    t.qpos[r0:r1] = t.rng.permutation(t.qpos[r0:r1])
+    t.qpos[r0 + 3] = 0
+    t.qpos[2:t.row0[-1]:13] = NONE
+    t.qpos[t.row0[4]:t.row0[5]] = NONE
+    only = [0, heads // kv // 2, heads // kv, heads - 1]
+    got = check_attention(kernels, stream, t.device(), heads, gate=gate, only=only)
+    again = run_attention(kernels, stream, t, heads, gate=gate)[0]
+    assert np.array_equal(again, got)
+    # sequence 7: V's scale of tokens 32 .. 47 of kv head 0 is NaN; a page of sequence 2 that is none
+    t.host[0].s[t.table[7, 0], 0, 1, 2] = np.nan
+    page, t.table[2, 4] = t.table[2, 4], t.pages
+    want = np.zeros((t.rows, heads), bool)
+    seen = (t.qpos + np.uint32(1)).astype(np.int64)
+    for s, start, of in ((7, 32, heads // kv), (2, 256, heads)):
+        r = slice(int(t.row0[s]), int(t.row0[s + 1]))
+        want[r, :of] = (seen[r] > start)[:, None]
+    t.device()
+    t.table[2, 4] = page
+    bad = check_attention(kernels, stream, t, heads, gate=gate, only=only, nan=want)
+    nan = np.isnan(bad.astype(np.float64))
+    assert np.array_equal(nan.all(-1), want) and np.array_equal(nan.any(-1), want)
+    if fmt == "e4m3":  # scales are powers of two: which one weights are taken relative to moves no bit
+        assert np.array_equal(bad[~want], got[~want])
+
+
+@pytest.mark.parametrize("fmt,heads,kv,dim,lens,counts", [
+    ("e4m3", 12, 2, 128, [5000, 700, 64], [250, 30, 1]), ("int8", 8, 1, 128, [9000], [70]),
+    ("int8", 8, 1, 256, [4200, 900], [110, 40]), ("e4m3", 16, 4, 256, [7001, 4099], [130, 150])])
+def test_attention_of_chunks_behind_long_sequences(gpu, kernels, stream, fmt, heads, kv, dim, lens, counts):
+    """Some hundred rows over thousands of tokens: tiles of 128 in runs, their states merged; a sequence whose rows see
+    nothing, rows in no order. Another stream's workspace, sized for more rows and tokens beforehand, gives the same bits."""
+    t = Setup(kv, dim, fmt, lens, counts, seed=dim + heads, layers=1, layer=0)
+    t.fill(lens)
+    r0, r1 = int(t.row0[0]), int(t.row0[1])
+    t.qpos[r0:r1] = t.rng.permutation(t.qpos[r0:r1])
+    t.qpos[r0 + 1] = 20
+    t.qpos[2:t.row0[-1]:13] = NONE
+    t.qpos[t.row0[2] if len(lens) > 2 else t.rows:] = NONE
+    got = check_attention(kernels, stream, t.device(), heads, only=[0, heads // kv - 1, heads - 1])
+    s = Stream()
+    kernels.kv8.attention_ws(s.handle, t.cache, 2 * t.rows, len(lens), heads, 2 * max(lens))
+    again = run_attention(kernels, s.handle, t, heads)[0]
+    s.synchronize()
+    assert np.array_equal(again, got)
+    s.destroy()
+
+
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("scale", [0.0, -0.125, 2.0])
 def test_attention_scales_and_sharp_weights(gpu, kernels, stream, fmt, scale):
@@ -447,6 +510,29 @@ def test_attention_makes_rows_that_see_a_bad_page_nan(gpu, kernels, stream, rows
     seen = t.qpos[:2 * rows] + 1
     assert np.array_equal(nan[:rows].all((1, 2)), seen[:rows] > 128) and np.array_equal(nan[:rows].any((1, 2)), seen[:rows] > 128)
     assert np.array_equal(nan[rows:2 * rows].all((1, 2)), seen[rows:] > 256)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("garbage", [np.nan, np.inf, 3e38])
+@pytest.mark.parametrize("rows", [8, 120, 500])
+def test_attention_keeps_a_bad_page_from_rows_that_do_not_see_it(gpu, kernels, stream, rows, garbage, fmt):
+    """Whatever the unused pages hold: NaN codes, scales that are not finite or huge."""
+    t = Setup(4, 128, fmt, [1000], [rows], layers=1, layer=0, seed=rows, pages=40)
+    t.table[0, :16] = np.arange(1, 17)  # page 0 is not used
+    t.fill([1000])
+    t.host[0].s[0] = garbage
+    got = run_attention(kernels, stream, t.device(), 32)[0]
+    first = 14 if rows > 8 else 15  # the bad page: rows before and behind its start, or its inside
+    if rows == 8:
+        t.qpos[:8] = np.arange(956, 964)
+        got = run_attention(kernels, stream, t.device(), 32)[0]
+    t.table[0, first] = 0xFFFFFFFF
+    bad = run_attention(kernels, stream, t.device(), 32)[0].astype(np.float64)
+    sees = t.qpos[:rows] >= 64 * first
+    assert sees.any() and not sees.all()
+    assert np.isnan(bad[:rows][sees]).all() and np.isfinite(bad[:rows][~sees]).all()
+    good = got[:rows][~sees].astype(np.float64)
+    assert (np.abs(bad[:rows][~sees] - good) <= 2.0 ** -8 * (np.abs(good) + 1)).all()
 
 
 def test_attention_reads_pages_past_4_gib(gpu, kernels, stream):
