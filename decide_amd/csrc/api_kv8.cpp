@@ -62,6 +62,8 @@ int check_cache(const char* op, const dh_kv8_cache* c) {
   return DH_OK;
 }
 
+constexpr uint64_t kMaxThreads = UINT32_MAX;  // of a launch, in a dimension
+
 int check_batch(const char* op, const dh_kv8_batch* b) {
   if (!b) return fail(DH_EINVAL, "%s: null batch", op);
   if (b->rows && b->seqs && (!b->table || !b->row0 || !b->qpos)) return fail(DH_EINVAL, "%s: null pointer in the batch", op);
@@ -83,10 +85,10 @@ int check_heads(const char* op, const dh_kv8_cache* c, uint32_t heads) {
   return DH_OK;
 }
 
-// Work items are numbered in 32 bits, and a grid holds 2^31 - 1 workgroups.
+// Work items are numbered in 32 bits; a tile's merge takes up to four workgroups.
 int check_attention_size(const char* op, const dh_kv8_cache* c, uint32_t rows, uint32_t seqs, uint32_t heads) {
   const uint64_t tiles = ((uint64_t)rows * (heads / c->kv_heads)) / 16 + seqs;
-  if ((uint64_t)rows * heads > UINT32_MAX || tiles * c->kv_heads * 4 > INT32_MAX)
+  if ((uint64_t)rows * heads > UINT32_MAX || tiles * c->kv_heads * 4 > kMaxThreads / 512)
     return fail(DH_EINVAL, "%s: %u rows x %u heads over %u sequences exceed one launch; split the call", op, rows, heads,
                 seqs);
   return DH_OK;
@@ -112,7 +114,7 @@ int dh_rope(dh_ctx* ctx, void* stream, const void* x, uint32_t ldx, uint32_t x_d
   if (rc == DH_OK) rc = check_rows("rope", "y", y, ldy, y_dtype, wide);
   if (rc != DH_OK) return rc;
   if (misaligned(pos, 4)) return fail(DH_EINVAL, "rope: pos must be 4-byte aligned");
-  if (rows > INT32_MAX) return fail(DH_EINVAL, "rope: %u rows exceed one launch; split the call", rows);
+  if (rows > kMaxThreads / 256) return fail(DH_EINVAL, "rope: %u rows exceed one launch; split the call", rows);
   if (x && x == y && (x_dtype != y_dtype || ldx != ldy))
     return fail(DH_EINVAL, "rope: y may be x only with its dtype and row stride");
   if (!ctx) return fail(DH_EINVAL, "rope: null context");
@@ -164,8 +166,9 @@ int dh_kv8_append(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, uint32_t
   rc = check_rows("kv8_append", "k", k, ldk, dtype, wide);
   if (rc == DH_OK) rc = check_rows("kv8_append", "v", v, ldv, dtype, wide);
   if (rc != DH_OK) return rc;
-  if ((uint64_t)batch->rows / DH_KV8_BLOCK + 2 * (uint64_t)batch->seqs > INT32_MAX)
-    return fail(DH_EINVAL, "kv8_append: %u sequences exceed one launch; split the call", batch->seqs);
+  if ((uint64_t)batch->rows / DH_KV8_BLOCK + 2 * (uint64_t)batch->seqs > kMaxThreads / 256)
+    return fail(DH_EINVAL, "kv8_append: %u rows of %u sequences exceed one launch; split the call", batch->rows,
+                batch->seqs);
   if (!ctx) return fail(DH_EINVAL, "kv8_append: null context");
   if (batch->rows && batch->seqs && (!k || !v)) return fail(DH_EINVAL, "kv8_append: null pointer");
   mark(ctx, kKidKv8Append);
@@ -237,7 +240,8 @@ int dh_kv8_copy_pages(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, cons
   if (misaligned(src, 4) || misaligned(dst, 4))
     return fail(DH_EINVAL, "kv8_copy_pages: src and dst must be 4-byte aligned");
   const uint64_t bytes = dh_kv8_page_bytes(cache->kv_heads, cache->head_dim);
-  if ((bytes / 16384 + 1) * (uint64_t)std::min(n, cache->pages) > INT32_MAX / (uint64_t)cache->layers || n > cache->pages)
+  if ((bytes / 16384 + 1) * (uint64_t)std::min(n, cache->pages) > kMaxThreads / 256 / cache->layers ||
+      n > cache->pages)
     return fail(DH_EINVAL, "kv8_copy_pages: %u pairs for %u pages in %u layers exceed one launch", n, cache->pages,
                 cache->layers);
   if (!ctx) return fail(DH_EINVAL, "kv8_copy_pages: null context");
@@ -268,12 +272,14 @@ int kv8_warm(dh_ctx* ctx, hipStream_t s, void* mem) {
   int rc = dh_rope(ctx, s, x, 64, 2, y, 64, 0, u, 1, 1, &rope);
   if (rc == DH_OK) rc = dh_kv8_append(ctx, s, &cache, 0, &batch, x, 64, x, 64, 2, &rope);
   if (rc == DH_OK) {
-    dh::KvAttnPlan plan{1, 1, 8, false, 0};  // one run: the combine too
     mark(ctx, kKidKv8Attn);
     mark(ctx, kKidKv8Combine);
-    rc = hip_status(dh::launch_kv8_attention(kv_args(&cache, 0, &batch), 64, false, (const _Float16*)x, 64, 1, 1.f,
-                                             nullptr, 0, (_Float16*)y, 64, (float*)(base + 49152), plan, s),
-                    "kv8_attention");
+    // one run, with the combine; one wide tile
+    for (const dh::KvAttnPlan& plan : {dh::KvAttnPlan{1, 1, 8, false, 0}, dh::KvAttnPlan{1, 0, 0, true, 0}})
+      if (rc == DH_OK)
+        rc = hip_status(dh::launch_kv8_attention(kv_args(&cache, 0, &batch), 64, false, (const _Float16*)x, 64, 1, 1.f,
+                                                 nullptr, 0, (_Float16*)y, 64, (float*)(base + 49152), plan, s),
+                        "kv8_attention");
   }
   if (rc == DH_OK) rc = dh_kv8_copy_pages(ctx, s, &cache, u, u + 1, 0);
   return rc;

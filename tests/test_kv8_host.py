@@ -116,6 +116,15 @@ def test_copy_refusals(kw, msg):
     _refused(_copy(**kw), msg)
 
 
+@pytest.mark.parametrize("call,kw", [
+    (_rope, dict(rows=1 << 24)), (_append, dict(batch=dict(rows=1 << 28))), (_append, dict(batch=dict(seqs=1 << 23))),
+    (_attention, dict(batch=dict(rows=1 << 31))), (_attention, dict(batch=dict(seqs=1 << 22))),
+    (_copy, dict(cache=dict(pages=1 << 26), n=1 << 25))])
+def test_what_exceeds_one_launch_is_refused(call, kw):
+    """A launch's threads are counted in 32 bits; nothing is launched in part."""
+    _refused(call(**kw), "one launch")
+
+
 def test_null_descriptors_are_refused():
     lib = _lib.load()
     _refused(lib.dh_rope(None, None, 16, 64, 2, 16, 64, 2, 4, 1, 1, None), "null spec")
