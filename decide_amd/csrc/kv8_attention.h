@@ -2,6 +2,8 @@
 // (row, head) pairs, and the runs of pages that workgroups take. Device code only.
 #pragma once
 
+#include <type_traits>
+
 #include "kv8_device.h"
 
 namespace dh {
@@ -49,9 +51,17 @@ __device__ __forceinline__ float sum_groups(float x) {
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
-  return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+  auto with = [&](auto lanes) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, decltype(lanes)::value, 0xf, 0xf, false));
+  };
+  with(std::integral_constant<int, 0xb1>{});   // the neighbour's
+  with(std::integral_constant<int, 0x4e>{});   // the neighbouring pair's
+  with(std::integral_constant<int, 0x141>{});  // mirrored within 8 lanes: the other four's
+  with(std::integral_constant<int, 0x140>{});  // within 16: the other eight's
+  auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(a[0], a[1]);
+  a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)max(a[0], a[1]));
 }
 
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + __expf(-x)); }
@@ -106,7 +116,8 @@ __device__ __forceinline__ void pair_at(const AttnArgs& t, const Tile& tile, uin
 
 // Pages of `seen` tokens. One page past the table is enough to make the row NaN.
 __device__ __forceinline__ uint32_t pages_of(const KvArgs& a, uint32_t seen) {
-  return min(seen / kKvPage + (seen % kKvPage != 0), a.ld_table + 1);
+  const uint32_t n = seen / kKvPage + (seen % kKvPage != 0);  // at most 2^26
+  return n > a.ld_table ? a.ld_table + 1 : n;
 }
 
 // The runs: run w of `share` pages each, over the tiles' pages one after another.
@@ -197,6 +208,9 @@ __device__ __forceinline__ void deal_runs(const KvArgs& a, const AttnArgs& t, ui
   u = (uint32_t)min((uint64_t)run * share, (uint64_t)total);
   u1 = min(u + share, total);
 }
+
+// A value that all lanes have, in a scalar register.
+__device__ __forceinline__ uint32_t same(uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); }
 
 // The tile that holds page u of a kv head: the last that starts at or before it (empty ones start where the next does).
 template <uint32_t SLOTS>

@@ -48,24 +48,20 @@ __global__ __launch_bounds__(512) void kv8_attention_kernel(KvArgs a, AttnArgs t
     uint32_t slot = run, tile_u = 0;
     Tile tile;
     if constexpr (RUNS) {
-      slot = tile_at(deal, t.slots, u);
-      tile_u = deal.before[slot];
-      const uint32_t q0 = deal.seq[slot];
+      slot = same(tile_at(deal, t.slots, u));
+      tile_u = same(deal.before[slot]);
+      const uint32_t q0 = same(deal.seq[slot]);
       // (it has pages, so it has rows)
-      if (!tile_of<kKvTile>(a, t.group, slot, q0, deal.row0[q0], deal.row0[q0 + 1], tile)) return;
+      if (!tile_of<kKvTile>(a, t.group, slot, q0, same(deal.row0[q0]), same(deal.row0[q0 + 1]), tile)) return;
     } else if (!find_tile<kKvTile>(a, t.group, slot, tile)) {
       return;
     }
     uint32_t row, head;
     pair_at(t, tile, kvh, min(n, tile.pairs - 1), row, head);
     const uint32_t seen = seen_by(a, row);
-    const uint32_t most = wave_max_u32(seen);
-    const uint32_t least = ~wave_max_u32(~seen);
-    const uint32_t npages = pages_of(a, most);
-    const uint32_t b0 = u - tile_u, b1 = RUNS ? min(npages, u1 - tile_u) : npages;
-    if (RUNS && b1 <= b0) return;  // positions that changed under the call
-    const bool whole = !RUNS || (b0 == 0 && b1 == npages);
     const uint32_t* const table = a.table + (size_t)tile.seq * a.ld_table;
+    auto id_of = [&](uint32_t b) { return b < a.ld_table ? table[b] : 0xffffffffu; };
+    uint32_t next = id_of(u - tile_u + wave);  // with the position and Q, not behind them; later ids a page ahead
 
     // Q: dims 64 j + 16 g + 8 e .. + 7 of pair n
     h8 q[2 * S];
@@ -76,10 +72,16 @@ __global__ __launch_bounds__(512) void kv8_attention_kernel(KvArgs a, AttnArgs t
         q[2 * j] = *(const h8*)(qp + 64 * j);
         q[2 * j + 1] = *(const h8*)(qp + 64 * j + 8);
       }
-      if (t.scale < 0.f) {
+    }
+    const uint32_t most = wave_max_u32(seen);
+    const uint32_t least = ~wave_max_u32(~seen);
+    const uint32_t npages = pages_of(a, most);
+    const uint32_t b0 = u - tile_u, b1 = RUNS ? min(npages, u1 - tile_u) : npages;
+    if (RUNS && b1 <= b0) return;  // positions that changed under the call
+    const bool whole = !RUNS || (b0 == 0 && b1 == npages);
+    if (t.scale < 0.f) {
 #pragma unroll
-        for (int j = 0; j < 2 * S; ++j) q[j] = -q[j];
-      }
+      for (int j = 0; j < 2 * S; ++j) q[j] = -q[j];
     }
     // the gate of the thread's first four outputs, in flight through the pages
     const uint32_t pairs = min(kKvTile, tile.pairs);
@@ -96,7 +98,8 @@ __global__ __launch_bounds__(512) void kv8_attention_kernel(KvArgs a, AttnArgs t
     float vref = 0x1p-100f, inv_vref = 0x1p100f;  // the largest V scale met; o is relative to it
 
     for (uint32_t b = b0 + wave; b < b1; b += kWaves) {
-      const uint32_t id0 = b < a.ld_table ? table[b] : 0xffffffffu;
+      const uint32_t id0 = next;
+      next = id_of(b + kWaves);
       const bool bad = id0 >= a.pages;
       const uint8_t* const rec = a.pool + (bad ? 0 : id0) * a.page_bytes;
       const uint8_t* const kp = rec + kv_k_at<D>(kvh) + ktok * D + 16 * g;

@@ -512,6 +512,17 @@ def test_attention_makes_rows_that_see_a_bad_page_nan(gpu, kernels, stream, rows
     assert np.array_equal(nan[rows:2 * rows].all((1, 2)), seen[rows:] > 256)
 
 
+@pytest.mark.parametrize("rows", [3, 700])
+def test_attention_over_one_table_of_any_stated_length(gpu, kernels, stream, rows):
+    """One sequence's table may be said to be as long as 32 bits count: only entries at the seen pages are read (and the few
+    behind them that are there)."""
+    t = Setup(2, 128, "e4m3", [rows + 30], [rows], layers=1, layer=0, seed=rows, wide=40)
+    t.fill([rows + 30])
+    t.device()
+    t.batch = Kv8Batch((u32(t.table), 0), 0xFFFFFFFF, (u32(t.row0), 0), (u32(t.qpos), 0), 1, t.rows)
+    check_attention(kernels, stream, t, 32, only=[0, 17])
+
+
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("garbage", [np.nan, np.inf, 3e38])
 @pytest.mark.parametrize("rows", [8, 120, 500])
