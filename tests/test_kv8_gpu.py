@@ -199,6 +199,31 @@ def test_append_codes_rows_as_defined(gpu, kernels, stream, kv, dim, dtype, fmt,
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("kv,dim,dtype,turned", [(17, 64, "f32", True), (33, 64, "bf16", False), (16, 128, "f16", True),
+                                                 (15, 256, "f32", False)])
+def test_append_of_many_sequences_and_heads(gpu, kernels, stream, kv, dim, dtype, turned, fmt):
+    """More blocks of tokens and heads than run at once: a workgroup takes several heads, the last one fewer."""
+    lens, counts = [5 + 3 * i for i in range(70)], [1 + i % 4 for i in range(70)]
+    t = Setup(kv, dim, fmt, lens, counts, seed=kv, layers=1, layer=0)
+    t.fill([n - c for n, c in zip(lens, counts)])
+    t.device()
+    wide = kv * dim
+    raw, x = to_type(t.rng.standard_normal((t.rows, 2 * wide)) * 3.0, dtype)
+    freq, d = np.array(rope_freqs(dim, 1e4)[0], np.float32), to_dev(raw)
+    fd = to_dev(freq)
+    kernels.kv8.append(stream, t.cache, 0, t.batch, (d, 0), 2 * wide, (d, wide * raw.itemsize), 2 * wide, dtype,
+                       RopeSpec((fd, 0), dim, dim) if turned else None)
+    sync()
+    k, v = (x[:, i * wide:(i + 1) * wide].reshape(-1, kv, dim) for i in (0, 1))
+    if turned:
+        pos = np.zeros(t.rows)
+        pos[:t.row0[-1]] = t.qpos[:t.row0[-1]]
+        k = ref.rope(k, pos, freq, 1.0, dim, "half")
+    t.host[0].append(t.table, t.row0, t.qpos, k.astype(np.float32), v.astype(np.float32))
+    same_pool(t, t.host)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("dim,rot,layout,norm", [(256, 64, "half", True), (128, 128, "interleaved", True),
                                                  (64, 30, "half", False), (64, 64, "half", True)])
 def test_append_turns_keys_in_64_bits(gpu, kernels, stream, fmt, dim, rot, layout, norm):
