@@ -254,6 +254,25 @@ __device__ __forceinline__ float state_weight(float m, float top) {
   return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
 }
 
+// V's scales differ from block to block, so what a pair rounds to fp16 is the product of a token's weight and its block's
+// scale, relative to `vref`: at least the largest block's share (its largest weight times its scale) over 2^8 among the
+// blocks that this pair sees, and at most the largest. So the products stay at most 2^8, and each is off by 2^-11 of
+// itself or 2^-25 of the largest share, whatever scales unseen blocks or those of next to no weight have. Relative to the
+// largest scale alone, a block of values 2^20 larger behind a row's position took 5 % of that row.
+constexpr float kNoScale = 0x1p-100f;   // no block's scale is smaller
+constexpr float kMostScale = 0x1p126f;  // vref's, and a ratio's, largest: the reciprocal and the products stay finite
+__device__ __forceinline__ float block_share(float top, float m, float vs) {
+  return __builtin_amdgcn_exp2f(top - (m == -INFINITY ? 0.f : m)) * vs;
+}
+// Whether a page whose largest score and share are bm and vm moves the pair's reference points.
+__device__ __forceinline__ bool moves(float bm, float m, float vm, float vref) {
+  return bm > m + kLazy || vm > 256.0f * vref;
+}
+__device__ __forceinline__ float scale_ratio(float vs, float vref) {
+  const float r = vs * __builtin_amdgcn_rcpf(vref);  // off by 2^-23 at most
+  return r > kMostScale ? kMostScale : r;  // (where weights vanish; a NaN scale stays)
+}
+
 // kv8_wide.hip: the kernel for many rows, over t.runs runs or t.slots tiles
 hipError_t launch_kv8_wide(const KvArgs& a, const AttnArgs& t, uint32_t head_dim, bool int8, hipStream_t s);
 

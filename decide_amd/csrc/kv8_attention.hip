@@ -9,9 +9,8 @@
 //     V lies transposed in the page, so the other operand's 16 tokens are 16 consecutive bytes. Nothing of K, V, S or P
 //     goes through LDS.
 //   * Codes become fp16 exactly (e4m3: one conversion for two; int8: a byte next to 0x64 is 1024 + b as fp16, then one
-//     subtraction for two). The K scale joins the softmax's factor; the V scale, relative to the largest that the wave
-//     has met, multiplies the weight in fp32 before its rounding to fp16, so weights stay at most 2^8 and one page's small
-//     scale cannot push another's weights out of fp16's range.
+//     subtraction for two). The K scale joins the softmax's factor; the V scale multiplies the weight in fp32 before its
+//     rounding to fp16, relative to the largest such product that the pair has met (block_share in kv8_attention.h).
 //   * The eight waves of a workgroup take every eighth page and meet at the end of a tile, through LDS.
 //   * Sequences of one call may differ in length by any factor, and the host does not know them. So the workgroups of a
 //     kv head (one per CU in all) add up the pages of all tiles, each for itself, and take equal runs of them: a run may
@@ -95,7 +94,7 @@ __global__ __launch_bounds__(512) void kv8_attention_kernel(KvArgs a, AttnArgs t
 #pragma unroll
     for (int i = 0; i < DT; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
-    float vref = 0x1p-100f, inv_vref = 0x1p100f;  // the largest V scale met; o is relative to it
+    float vref = kNoScale;  // what the pair's o is relative to
 
     for (uint32_t b = b0 + wave; b < b1; b += kWaves) {
       const uint32_t id0 = next;
@@ -152,25 +151,27 @@ __global__ __launch_bounds__(512) void kv8_attention_kernel(KvArgs a, AttnArgs t
           }
         }
       }
-      float bm = sv[0];
+      float top = sv[0];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) bm = fmaxf(bm, sv[i]);
-      bm = max_groups(bm * unit);
-      const float vm = max_groups(vs);  // the same in every lane
-      if (__any(bm > m + kLazy) || vm > vref) {
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, sv[i]);
+      top *= unit;  // of the lane's block
+      const float bm = max_groups(top);
+      auto share = [&](float ref) { return max_groups(blind ? 0.f : block_share(top, ref, vs)); };
+      const float vm = share(m);
+      if (__any(moves(bm, m, vm, vref))) {
+        const bool mine = moves(bm, m, vm, vref);  // a pair's own: the others of the tile keep their bits
         const float mnew = bm > m + kLazy ? bm : m;
-        const float alpha = state_weight(m, mnew);
-        const float vnew = fmaxf(vref, vm);
+        const float alpha = state_weight(m, mnew), vold = alpha * vref;
+        const float vnew = mine ? fminf(fmaxf(vold, share(mnew)), kMostScale) : vref;
+        const float both = mine ? vold / vnew : 1.0f;
         l *= alpha;
         m = mnew;
-        const float both = alpha * (vref / vnew);
         vref = vnew;
-        inv_vref = 1.0f / vnew;
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[i] *= both;
       }
       const float mref = m == -INFINITY ? 0.f : m;
-      const float ratio = blind ? 0.f : vs * inv_vref;
+      const float ratio = blind ? 0.f : scale_ratio(vs, vref);
       h8 p[2];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {

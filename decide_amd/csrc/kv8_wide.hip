@@ -76,10 +76,10 @@ __global__ __launch_bounds__(512) void kv8_attention_wide_kernel(KvArgs a, AttnA
     uint32_t slot = t.slots - 1 - run, tile_u = 0;  // one tile each: the last, longest ones first
     Tile tile;
     if constexpr (RUNS) {
-      slot = tile_at(deal, t.slots, u);
-      tile_u = deal.before[slot];
-      const uint32_t q0 = deal.seq[slot];
-      if (!tile_of<kKvWideTile>(a, t.group, slot, q0, deal.row0[q0], deal.row0[q0 + 1], tile)) return;
+      slot = same(tile_at(deal, t.slots, u));
+      tile_u = same(deal.before[slot]);
+      const uint32_t q0 = same(deal.seq[slot]);
+      if (!tile_of<kKvWideTile>(a, t.group, slot, q0, same(deal.row0[q0]), same(deal.row0[q0 + 1]), tile)) return;
     } else if (!find_tile<kKvWideTile>(a, t.group, slot, tile)) {
       return;
     }
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(512) void kv8_attention_wide_kernel(KvArgs a, AttnA
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
     float m = -INFINITY, l = 0.f;
-    float vref = 0x1p-100f, inv_vref = 0x1p100f;
+    float vref = kNoScale;
 
     auto id_of = [&](uint32_t b) { return b < b1 ? page_id(b) : 0; };
     uint32_t id0 = id_of(b0), id1 = id_of(b0 + 1), id2 = id_of(b0 + 2), id3 = id_of(b0 + 3);  // of pages b .. b + 3
@@ -225,26 +225,27 @@ __global__ __launch_bounds__(512) void kv8_attention_wide_kernel(KvArgs a, AttnA
           blind = mine == 0;
           if (tok0 >= most || bad) vs = 0.f;
         }
-        float bm = st[0];
+        float top = st[0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) bm = fmaxf(bm, st[i]);
-        bm = max_halves(bm * unit);
-        // the same in every lane: kept in scalar registers
-        const float vm = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(max_halves(vs))));
-        if (__any(bm > m + kLazy) || vm > vref) {
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, st[i]);
+        top *= unit;  // of the lane's block
+        const float bm = max_halves(top);
+        auto share = [&](float ref) { return max_halves(blind ? 0.f : block_share(top, ref, vs)); };
+        const float vm = share(m);
+        if (__any(moves(bm, m, vm, vref))) {
+          const bool mine = moves(bm, m, vm, vref);  // a pair's own: the others of the tile keep their bits
           const float mnew = bm > m + kLazy ? bm : m;
-          const float alpha = state_weight(m, mnew);
-          const float vnew = fmaxf(vref, vm);
+          const float alpha = state_weight(m, mnew), vold = alpha * vref;
+          const float vnew = mine ? fminf(fmaxf(vold, share(mnew)), kMostScale) : vref;
+          const float both = mine ? vold / vnew : 1.0f;
           l *= alpha;
           m = mnew;
-          const float both = alpha * (vref / vnew);
-          vref = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(vnew)));
-          inv_vref = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(1.0f / vnew)));
+          vref = vnew;
 #pragma unroll
           for (int i = 0; i < DT; ++i) o[i] *= both;
         }
         const float mref = m == -INFINITY ? 0.f : m;
-        const float ratio = blind ? 0.f : vs * inv_vref;
+        const float ratio = blind ? 0.f : scale_ratio(vs, vref);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float w = __builtin_amdgcn_exp2f(fmaf(st[i], unit, -mref));

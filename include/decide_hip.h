@@ -625,10 +625,12 @@ int dh_kv8_append(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, uint32_t
  * over tokens t = 0 ..= qpos[r] of row r's sequence, kv head g = h / (heads /
  * kv_heads); a row without a position sees no token and its y is zero. q fp16
  * [rows, heads * head_dim] row stride ldq, y fp16 row stride ldy, gate (may be
- * NULL) fp32 row stride ldg; scores and softmax fp32, the weights rounded to
- * fp16 as the operand of their product with V. max_tokens: how many tokens the
- * longest row sees, for the launch's division of long sequences; a row may see
- * more (slower) or all fewer. Rows in any order of positions.
+ * NULL) fp32 row stride ldg; scores and softmax fp32; the products of a weight
+ * and its block's V scale, relative to the largest that the row meets, are
+ * rounded to fp16 as the operand of their product with V's codes. max_tokens:
+ * how many tokens the longest row sees, for the launch's division of long
+ * sequences; a row may see more (slower) or all fewer. Rows in any order of
+ * positions.
  * A row that sees a token whose page id is not below cache->pages, or whose
  * table entry would lie past ld_table, is NaN; so is one that sees a token of a
  * block with a NaN scale. Bytes behind a sequence's last seen token may hold

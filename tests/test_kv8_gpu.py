@@ -841,3 +841,84 @@ def test_nothing_new_is_loaded_after_warm_up(gpu, kernels, stream):
     t.device()
     check_attention(kernels, stream, t, 4)
     assert kernels.gemm.fast_pipelines() == n
+
+
+# ---- V scales that differ by many powers within a sequence ----------------------------------------------------------
+def uneven(layout, rows, small, ahead, power, far, seed):
+    """(a cache layer of one sequence, its queries): `small` tokens of values near 2^-12, then a block whose
+    values are 2^power times larger and whose keys lie 2^-far below in weight for every query (`far` 0: like the others).
+    Rows stand before, at and behind the block's start in turn; `ahead`: the large block comes first."""
+    fmt, heads, kv, dim = layout
+    n = small + 16
+    t = Setup(kv, dim, fmt, [n], [rows], layers=1, layer=0, seed=seed)
+    k = t.rng.standard_normal((n, kv, dim)).astype(np.float32) * 0.25
+    v = t.rng.standard_normal((n, kv, dim)).astype(np.float32) * np.float32(2.0 ** -12)
+    big = slice(0, 16) if ahead else slice(small, n)
+    v[big] *= np.float32(2.0 ** power)
+    q = (t.rng.standard_normal((t.rows, heads * dim + 16)) * 0.25).astype(np.float16)
+    if far:
+        q[:, 8::dim] = 8.0
+        k[:, :, 0] = 0.0
+        k[big, :, 0] = -far * np.log(2.0) / (8.0 * dim ** -0.5)
+    t.host[0].append(t.table, np.array([0, n]), np.arange(n), k, v)
+    t.qpos[:rows] = (np.arange(rows) * 5 % 32 + n - 32 if not ahead else 16 + np.arange(rows) * 7 % (n - 16)).astype(np.uint32)
+    return t, q
+
+
+def uneven_bound(t, n, kh, vh, qv, p, want, fmt, g):
+    """attention_bound, with the subnormal weights' share relative to the largest product of a block's weight and its scale:
+    weights are held as weight x scale / (at least the largest such product / 2^8), so each is off by half of fp16's smallest
+    step, 2^-25, times that product and its code."""
+    sc = np.repeat(t.host[0].s[t.table[0, :-(-n // ref.PAGE)], g, 1].astype(np.float64).ravel(), ref.BLOCK)[:n]
+    code = 448.0 if fmt == "e4m3" else 127.0
+    size = p @ np.abs(vh)
+    err = 2 * (len(qv) + 2) * U * float(np.max(np.abs(kh) @ np.abs(qv))) * t.dim ** -0.5
+    return ((2.0 ** -11 + err + 2.0 ** -20) * size + n * 2.0 ** -25 * code * (p * sc).max() + 2.0 ** -11 * np.abs(want)
+            + 2.0 ** -25)
+
+
+def check_uneven(t, got, q, n, heads, fmt):
+    """Some 40 of the rows, the first and the last head, over the sequence's n tokens."""
+    k, v = t.host[0].tokens(t.table[0, :-(-n // ref.PAGE)], n)
+    rows, worst = int(t.row0[1]), 0.0
+    for r in range(0, rows, max(1, rows // 40)):
+        m = int(t.qpos[r]) + 1
+        for h in (0, heads - 1):
+            g = h // (heads // t.kv)
+            sc = k[:m, g] @ q[r, h] * t.dim ** -0.5
+            p = np.exp(sc - sc.max())
+            p /= p.sum()
+            want = p @ v[:m, g]
+            bound = uneven_bound(t, m, k[:m, g], v[:m, g], q[r, h], p, want, fmt, g)
+            worst = max(worst, float((np.abs(got[r, h].astype(np.float64) - want) / bound).max()))
+    assert worst <= 1.0, worst
+
+
+UNEVEN = [("narrow", 5, 8, 2, 128), ("narrow", 9, 4, 1, 256), ("narrow", 40, 6, 3, 64), ("wide", 330, 32, 4, 128),
+          ("wide", 260, 40, 4, 256), ("wide", 650, 64, 4, 64)]
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("power", [16, 20, 26])
+@pytest.mark.parametrize("small", [16, 592, 4112])
+@pytest.mark.parametrize("which,rows,heads,kv,dim", UNEVEN)
+def test_attention_of_rows_before_and_behind_a_large_block(gpu, kernels, stream, which, rows, heads, kv, dim, small, power,
+                                                           fmt):
+    """Rows of one tile, some of which see a block of values 2^power larger than all before it: the others are held
+    to their own tokens' values, whatever their neighbours see."""
+    t, q = uneven((fmt, heads, kv, dim), rows, small, False, power, 0, small + power)
+    got, _, qv, _ = run_attention(kernels, stream, t.device(), heads, gate=False, q=q)
+    check_uneven(t, got, qv, small + 16, heads, fmt)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("ahead", [False, True])
+@pytest.mark.parametrize("small", [32, 592, 4112])
+@pytest.mark.parametrize("which,rows,heads,kv,dim", UNEVEN)
+def test_attention_over_a_large_block_that_weighs_next_to_nothing(gpu, kernels, stream, which, rows, heads, kv, dim, small,
+                                                                  ahead, fmt):
+    """A block of values 2^26 larger that is seen with weights 2^-34 of the others': its share is 2^-8, and it takes nothing
+    from theirs."""
+    t, q = uneven((fmt, heads, kv, dim), rows, small, ahead, 26, 34.0, small)
+    got, _, qv, _ = run_attention(kernels, stream, t.device(), heads, gate=False, q=q)
+    check_uneven(t, got, qv, small + 16, heads, fmt)
