@@ -312,6 +312,19 @@ uint64_t least_pages(bool wide, uint32_t head_dim) {
   return wide ? 64 : head_dim == 256 ? 17 : head_dim == 128 ? 25 : 57;
 }
 
+// Many rows: tiles of 128 pairs. 16 heads over 4 of 256: 496 causal rows 33 us against 25 with tiles of 16, 603 rows 32
+// against 32, 1,000 rows 44 against 54, 8 x 128 rows 46 against 70; 32 over 8 of 128: 256 rows behind 544 tokens 25
+// against 18, 496 rows 22 against 26. Heads of 64 dims leave the narrow kernel room for two workgroups a CU: 8 heads over
+// one, 1,500 causal rows 30 against 14, 4,000 rows 69 against 54, 8,000 rows 141 against 155, 16 x 512 rows behind 2,000
+// tokens 61 against 84. Few rows behind many tokens, where the narrow kernel reads them once for every 16 pairs: 256 rows
+// of 4 heads behind 7,744 tokens 72 against 91, 128 rows behind 3,972 tokens 48 against 44.
+// More pairs, fewer sequences and more pages only ever turn to wide tiles.
+bool wide_tiles(uint64_t pairs, uint32_t seqs, uint32_t kv_heads, uint32_t head_dim, uint64_t pages, uint32_t cus) {
+  const uint64_t full = pairs / kKvTile * kv_heads;  // narrow tiles that are surely full
+  if (head_dim == 64) return full >= 10ull * cus;
+  return full >= 5ull * cus / 2 || (pages >= least_pages(true, head_dim) && pairs >= 512ull * seqs);
+}
+
 // Two states for each run, and where each slot's runs start.
 uint64_t run_bytes(bool wide, uint64_t runs, uint64_t slots, uint32_t kv_heads, uint32_t head_dim) {
   return (kv_heads * runs * 2 * ((wide ? kKvWideTile : kKvTile) * (head_dim + 2)) + slots + 1) * sizeof(float);
@@ -324,14 +337,7 @@ KvAttnPlan kv8_attention_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint
   const uint64_t pairs = (uint64_t)rows * (heads / kv_heads);
   const uint64_t pages = std::min<uint64_t>(((uint64_t)max_tokens + kKvPage - 1) / kKvPage, ld_table);
   const uint64_t full = pairs / kKvTile * kv_heads;  // narrow tiles that are surely full
-  // Many rows: tiles of 128 pairs. 16 heads over 4 of 256: 496 causal rows 33 us against 25 with tiles of 16, 603 rows 32
-  // against 32, 1,000 rows 44 against 54, 8 x 128 rows 46 against 70; 32 over 8 of 128: 256 rows behind 544 tokens 25
-  // against 18, 496 rows 22 against 26. Heads of 64 dims leave the narrow kernel room for two workgroups a CU: 8 heads over
-  // one, 1,500 causal rows 30 against 14, 4,000 rows 69 against 54, 8,000 rows 141 against 155, 16 x 512 rows behind 2,000
-  // tokens 61 against 84. Few rows behind many tokens, where the narrow kernel reads them once for every 16 pairs: 256 rows
-  // of 4 heads behind 7,744 tokens 72 against 91, 128 rows behind 3,972 tokens 48 against 44.
-  p.wide = head_dim == 64 ? full >= 10ull * cus
-                          : full >= 5ull * cus / 2 || (pages >= least_pages(true, head_dim) && pairs >= 512ull * seqs);
+  p.wide = wide_tiles(pairs, seqs, kv_heads, head_dim, pages, cus);
   const uint32_t tile = p.wide ? kKvWideTile : kKvTile;
   const uint64_t slots = pairs / tile + seqs;
   p.slots = (uint32_t)slots;
@@ -349,12 +355,13 @@ KvAttnPlan kv8_attention_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint
   return p;
 }
 
-// What any call of at most these sizes takes.
+// What any call of at most these sizes takes: in runs, wide tiles if such a call may have them.
 uint64_t kv8_attention_ws_bytes(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_tokens,
                                 uint32_t cus) {
   const uint64_t pages = ((uint64_t)max_tokens + kKvPage - 1) / kKvPage;
   if (pages < least_pages(false, head_dim)) return 0;
-  const bool wide = head_dim != 64 && pages >= least_pages(true, head_dim) && (uint64_t)rows * (heads / kv_heads) >= 512;
+  const bool wide = head_dim != 64 && pages >= least_pages(true, head_dim) &&
+                    wide_tiles((uint64_t)rows * (heads / kv_heads), 1, kv_heads, head_dim, pages, cus);
   return run_bytes(wide, std::max<uint32_t>(1, cus / kv_heads), kKvMaxSlots, kv_heads, head_dim);
 }
 

@@ -922,3 +922,43 @@ def test_attention_over_a_large_block_that_weighs_next_to_nothing(gpu, kernels, 
     t, q = uneven((fmt, heads, kv, dim), rows, small, ahead, 26, 34.0, small)
     got, _, qv, _ = run_attention(kernels, stream, t.device(), heads, gate=False, q=q)
     check_uneven(t, got, qv, small + 16, heads, fmt)
+
+
+@pytest.mark.parametrize("heads,kv,dim,rows", [(32, 32, 128, 400), (24, 24, 256, 432)])
+def test_a_capture_after_the_sizing_call_of_many_kv_heads(gpu, heads, kv, dim, rows):
+    """Many kv heads turn to tiles of 128 with fewer pairs a head: the sizing call holds what they take, and each replay has the
+    bits of an eager call on a stream of its own."""
+    import ctypes
+
+    kernels = Kernels()  # no workspace from another test
+    t = Setup(kv, dim, "int8", [4200], [rows], layers=1, layer=0, seed=kv, behind=0)
+    t.fill([4200])
+    t.device()
+    s, other = Stream(), Stream()
+    q, wide = to_dev(t.rng.standard_normal((rows, heads * dim)).astype(np.float16)), heads * dim
+    want, y = full((rows, wide), np.float16, 0), full((rows, wide), np.float16, 0)
+
+    def call(stream, to):
+        kernels.kv8.attention(stream, t.cache, 0, t.batch, (q, 0), wide, heads, dim ** -0.5, (to, 0), wide, 4200)
+
+    call(other.handle, want)
+    other.synchronize()
+    kernels.kv8.attention_ws(s.handle, t.cache, rows, 1, heads, 4200)
+    g, ge = ctypes.c_void_p(), ctypes.c_void_p()
+    check(rt().hipStreamBeginCapture(s.handle, 0), "begin")
+    try:
+        call(s.handle, y)
+    finally:
+        check(rt().hipStreamEndCapture(s.handle, ctypes.byref(g)), "end")
+    check(rt().hipGraphInstantiate(ctypes.byref(ge), g, None, None, 0), "instantiate")
+    for _ in range(3):
+        y.copy_from(np.zeros((rows, wide), np.float16))
+        check(rt().hipGraphLaunch(ge, s.handle), "launch")
+        s.synchronize()
+        assert np.array_equal(to_host(y), to_host(want)) and np.isfinite(to_host(y).astype(np.float32)).all()
+        call(other.handle, want)
+        other.synchronize()
+    check(rt().hipGraphExecDestroy(ge), "destroy")
+    check(rt().hipGraphDestroy(g), "destroy")
+    s.destroy()
+    other.destroy()

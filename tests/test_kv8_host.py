@@ -290,3 +290,42 @@ def test_reference_codes_are_the_nearest():
     assert np.abs(ref.values(ref.encode(x, "int8"), "int8") - x).max() <= 0.5
     assert ref.scale_of(448.0, "e4m3") == 1.0 and ref.scale_of(448.1, "e4m3") == 2.0
     assert ref.scale_of(0.0, "e4m3") == ref.FLOOR and ref.scale_of(224.0, "e4m3") == 0.5
+
+
+# ---- the attention's workspace --------------------------------------------------------------------------------------
+class _Plan(ctypes.Structure):
+    """``dh::KvAttnPlan`` (decide_amd/csrc/kv8.h)."""
+
+    _fields_ = [("slots", ctypes.c_uint32), ("runs", ctypes.c_uint32), ("min_run", ctypes.c_uint32),
+                ("wide", ctypes.c_bool), ("ws_bytes", ctypes.c_uint64)]
+
+
+def _attention_sizes():
+    """(plan of a call, bytes that the sizing call reserves): the library's own functions, by their linked names."""
+    lib = ctypes.CDLL(_lib.LIB_PATH)
+    plan = lib["_ZN2dh18kv8_attention_planEjjjjjjjj"]
+    plan.restype, plan.argtypes = _Plan, [ctypes.c_uint32] * 8
+    reserve = lib["_ZN2dh22kv8_attention_ws_bytesEjjjjjj"]
+    reserve.restype, reserve.argtypes = ctypes.c_uint64, [ctypes.c_uint32] * 6
+    return plan, reserve
+
+
+@pytest.mark.parametrize("cus", [256, 304, 64])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_the_reserved_workspace_covers_the_call_and_every_smaller_one(dim, cus):
+    plan, reserve = _attention_sizes()
+    r = random.Random(dim + cus)
+    sizes, runs, wide = 0, 0, 0
+    for kv in range(1, 129):
+        for group in (1, 2, 3, 8):
+            for rows in (1, 17, 80, 200, 320, 432, r.randint(1, 700)):
+                tokens = r.choice([5000, 8192, r.randint(1, 131072)])
+                held = reserve(rows, kv * group, kv, dim, tokens, cus)
+                for small in range(3):
+                    n, g = (rows, group) if small < 2 else (r.randint(1, rows), r.randint(1, group))
+                    t = tokens if small < 2 else r.randint(1, tokens)
+                    seqs = 1 if small == 0 else r.randint(1, n)
+                    p = plan(n, seqs, kv * g, kv, dim, r.choice([0xFFFFFF, tokens // 64 + 2]), t, cus)
+                    assert p.ws_bytes <= held, (kv, group, rows, tokens, n, g, t, seqs, p.wide, p.ws_bytes, held)
+                    sizes, runs, wide = sizes + 1, runs + (p.runs > 0), wide + (p.wide and p.runs > 0)
+    assert runs > sizes // 20 and (wide > 50 or dim == 64)  # the sweep meets what it is for
