@@ -74,7 +74,8 @@ bool forced_plan(const dh_ctx* c, int* variant, uint32_t* splits);
 int attention_run(dh_ctx* ctx, void* stream, const uint16_t* q, const uint16_t* kc, const uint16_t* vc,
                   const float* pq, const uint32_t* qpos, uint16_t* y, uint32_t rows, uint32_t ldq, uint32_t npos);
 
-// Launches every kernel of the 8-bit cache once on tiny inputs (dh_warm_up): `mem` holds kv8_warm_bytes() zeroed bytes.
+// Launches each kernel of the 8-bit cache once on tiny inputs (dh_warm_up), in one of its types and head sizes: code is
+// loaded by the source file, so the others come with it. `mem` holds kv8_warm_bytes() zeroed bytes.
 size_t kv8_warm_bytes();
 int kv8_warm(dh_ctx* ctx, hipStream_t s, void* mem);
 

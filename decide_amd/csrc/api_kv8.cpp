@@ -119,7 +119,7 @@ int dh_rope(dh_ctx* ctx, void* stream, const void* x, uint32_t ldx, uint32_t x_d
     return fail(DH_EINVAL, "rope: y may be x only with its dtype and row stride");
   if (!ctx) return fail(DH_EINVAL, "rope: null context");
   if (rows && heads && (!x || !y || !pos)) return fail(DH_EINVAL, "rope: null pointer");
-  mark(ctx, kKidRope);
+  if (rows && heads) mark(ctx, kKidRope);
   return hip_status(dh::launch_rope(x, ldx, x_dtype, y, ldy, y_dtype, pos, rows, heads, rope_args(spec),
                                     (hipStream_t)stream),
                     "rope");
@@ -171,7 +171,7 @@ int dh_kv8_append(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, uint32_t
                 batch->seqs);
   if (!ctx) return fail(DH_EINVAL, "kv8_append: null context");
   if (batch->rows && batch->seqs && (!k || !v)) return fail(DH_EINVAL, "kv8_append: null pointer");
-  mark(ctx, kKidKv8Append);
+  if (batch->rows && batch->seqs) mark(ctx, kKidKv8Append);
   return hip_status(dh::launch_kv8_append(kv_args(cache, layer, batch), cache->head_dim, cache->format == DH_KV8_INT8, k,
                                           ldk, v, ldv, dtype, rope_args(rope), (hipStream_t)stream),
                     "kv8_append");
@@ -246,7 +246,7 @@ int dh_kv8_copy_pages(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, cons
                 cache->layers);
   if (!ctx) return fail(DH_EINVAL, "kv8_copy_pages: null context");
   if (n && (!src || !dst)) return fail(DH_EINVAL, "kv8_copy_pages: null pointer");
-  mark(ctx, kKidKv8Copy);
+  if (n) mark(ctx, kKidKv8Copy);
   return hip_status(dh::launch_kv8_copy_pages((uint8_t*)cache->pool, bytes, cache->pages, cache->layers, src, dst, n,
                                               (hipStream_t)stream),
                     "kv8_copy_pages");
@@ -281,7 +281,7 @@ int kv8_warm(dh_ctx* ctx, hipStream_t s, void* mem) {
                                                  nullptr, 0, (_Float16*)y, 64, (float*)(base + 49152), plan, s),
                         "kv8_attention");
   }
-  if (rc == DH_OK) rc = dh_kv8_copy_pages(ctx, s, &cache, u, u + 1, 0);
+  if (rc == DH_OK) rc = dh_kv8_copy_pages(ctx, s, &cache, u, u, 1);  // page 0 onto itself
   return rc;
 }
 

@@ -962,3 +962,42 @@ def test_a_capture_after_the_sizing_call_of_many_kv_heads(gpu, heads, kv, dim, r
     check(rt().hipGraphDestroy(g), "destroy")
     s.destroy()
     other.destroy()
+
+
+def test_calls_without_work_count_no_kernel(gpu, stream):
+    """What dh_variants_loaded counts are launches: a call of no rows, heads, sequences or pairs is none."""
+    kernels = Kernels()
+    n = kernels.gemm.fast_pipelines()
+    t = Setup(1, 64, "e4m3", [10], [1], layers=1, layer=0).device()
+    x, f, ids = to_dev(np.zeros((4, 128), np.float32)), to_dev(np.ones(32, np.float32)), u32([0])
+    spec = RopeSpec((f, 0), 64, 64)
+    kernels.rope.rope(stream, (x, 0), 64, "f32", (x, 0), 64, "f32", (ids, 0), 0, 1, spec)
+    kernels.rope.rope(stream, (x, 0), 64, "f32", (x, 0), 64, "f32", (ids, 0), 1, 0, spec)
+    for rows, seqs in ((0, 1), (4, 0)):
+        b = Kv8Batch((u32(t.table), 0), t.table.shape[1], (u32(t.row0), 0), (u32(t.qpos), 0), seqs, rows)
+        kernels.kv8.append(stream, t.cache, 0, b, (x, 0), 128, (x, 256), 128, "f32")
+        kernels.kv8.attention(stream, t.cache, 0, b, (x, 0), 64, 1, 1.0, (x, 0), 64, 10)
+    kernels.kv8.copy_pages(stream, t.cache, (ids, 0), (ids, 0), 0)
+    sync()
+    assert kernels.gemm.fast_pipelines() == n
+
+
+def test_warm_up_covers_every_operator_of_the_cache(gpu, stream):
+    kernels = Kernels()
+    kernels.gemm.warm_up(stream, max_m=64)
+    n = kernels.gemm.fast_pipelines()
+    for kv, heads, rows, length in ((4, 16, 520, 540), (1, 4, 1, 5000)):  # tiles of 128; of 16, in runs
+        t = Setup(kv, 256, "int8", [length], [rows], layers=1, layer=0, seed=rows, behind=0)
+        t.fill([length])
+        t.device()
+        x = to_dev(t.rng.standard_normal((t.rows, 2 * kv * 256)).astype(np.float16))
+        f = to_dev(np.array(rope_freqs(64, 1e4)[0], np.float32))
+        spec = RopeSpec((f, 0), 256, 64, "interleaved")
+        q, y = full((t.rows, heads * 256), np.float16, 0.5), full((t.rows, heads * 256), np.float16, 0)
+        pos = u32(t.qpos)
+        kernels.rope.rope(stream, (q, 0), heads * 256, "f16", (y, 0), heads * 256, "f16", (pos, 0), t.rows, heads, spec)
+        kernels.kv8.append(stream, t.cache, 0, t.batch, (x, 0), 512 * kv, (x, 512 * kv), 512 * kv, "f16", spec)
+        kernels.kv8.attention(stream, t.cache, 0, t.batch, (q, 0), heads * 256, heads, 0.0625, (y, 0), heads * 256, length)
+        kernels.kv8.copy_pages(stream, t.cache, (u32([0]), 0), (u32([1]), 0), 1)
+        sync()
+    assert kernels.gemm.fast_pipelines() == n
