@@ -226,17 +226,21 @@ __device__ __forceinline__ uint32_t tile_at(const Deal<SLOTS>& d, uint32_t slots
   return lo;
 }
 
-// Four outputs of row r: O times `factor`, times the sigmoid of the gate where there is one.
-__device__ __forceinline__ void store_out(const AttnArgs& t, uint32_t r, uint32_t col, const f4& acc, float factor,
-                                          const f4& gate) {
-  f4 v = acc * factor;
-  if (t.gate) {
+// Four outputs of row r: O over its sum, times the sigmoid of the gate where there is one. A row that sees nothing is zero
+// whatever its gate; one that sees only scores of -infinity has the sum 0 and is NaN, as its softmax is.
+__device__ __forceinline__ void store_out(const AttnArgs& t, uint32_t r, uint32_t col, const f4& acc, float sum,
+                                          uint32_t sees, const f4& gate) {
+  f4 v = f4{0.f, 0.f, 0.f, 0.f};
+  if (sees) {
+    v = acc * (1.0f / sum);
+    if (t.gate) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] *= sigmoid(gate[e]);
+      for (int e = 0; e < 4; ++e) v[e] *= sigmoid(gate[e]);
+    }
   }
   *(h4*)(t.y + (size_t)r * t.ldy + col) = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
 }
-// eight dims, already over their sum
+// eight dims, already over their sum (zeros, and the gate one too, for a row that sees nothing)
 __device__ __forceinline__ void store_out8(const AttnArgs& t, uint32_t r, uint32_t col, f4 v0, f4 v1, const f4& g0,
                                            const f4& g1) {
   typedef _Float16 h8u __attribute__((ext_vector_type(8), aligned(8)));
@@ -247,7 +251,6 @@ __device__ __forceinline__ void store_out8(const AttnArgs& t, uint32_t r, uint32
   *(h8u*)(t.y + (size_t)r * t.ldy + col) = h8u{(_Float16)v0[0], (_Float16)v0[1], (_Float16)v0[2], (_Float16)v0[3],
                                                (_Float16)v1[0], (_Float16)v1[1], (_Float16)v1[2], (_Float16)v1[3]};
 }
-__device__ __forceinline__ float over_sum(float l) { return l == 0.f ? 0.f : 1.0f / l; }  // a row that sees nothing is 0
 
 // weight of a state whose reference point is m among those whose largest is top; none where it met no score
 __device__ __forceinline__ float state_weight(float m, float top) {

@@ -33,6 +33,7 @@ __global__ __launch_bounds__(512) void kv8_attention_kernel(KvArgs a, AttnArgs t
   constexpr int kWaves = 8;
   __shared__ __attribute__((aligned(16))) float lds[kWaves * kKvTile * kPad];
   __shared__ f2 ml[kWaves * kKvTile];
+  __shared__ uint32_t sees[kKvTile];  // how many tokens
   __shared__ Deal<RUNS ? kKvMaxSlots : 0> deal;
   const uint32_t kvh = blockIdx.x % a.kv_heads, run = blockIdx.x / a.kv_heads;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -189,6 +190,7 @@ __global__ __launch_bounds__(512) void kv8_attention_kernel(KvArgs a, AttnArgs t
     // The waves meet: each leaves its O relative to the largest of their reference points.
     l = sum_groups(l);
     if (g == 0) ml[wave * kKvTile + n] = f2{m, l};
+    if (tid < kKvTile) sees[n] = seen;
     __syncthreads();
     if (n < pairs) {
       float top = -INFINITY;
@@ -216,7 +218,7 @@ __global__ __launch_bounds__(512) void kv8_attention_kernel(KvArgs a, AttnArgs t
         uint32_t r, h;
         pair_at(t, tile, kvh, pr, r, h);
         if (t.gate && i != tid) gate = *(const f4*)(t.gate + (size_t)r * t.ldg + h * D + d);
-        store_out(t, r, h * D + d, acc, over_sum(lt), gate);
+        store_out(t, r, h * D + d, acc, lt, sees[pr], gate);
       } else {
         *(f4*)(state + pr * D + d) = acc;
         if (d == 0) *(f2*)(state + kKvTile * D + 2 * pr) = f2{top, lt};
@@ -251,6 +253,7 @@ __global__ __launch_bounds__(512) void kv8_combine_kernel(KvArgs a, AttnArgs t) 
   const uint32_t pr = min(PAIRS * part + item / L, tile.pairs - 1);
   uint32_t r, h;
   pair_at(t, tile, kvh, pr, r, h);
+  const uint32_t sees = seen_by(a, r);
   f4 gate = f4{0.f, 0.f, 0.f, 0.f};
   if (t.gate && way == 0) gate = *(const f4*)(t.gate + (size_t)r * t.ldg + h * D + d);  // with the states, not behind them
   f4 acc = f4{0.f, 0.f, 0.f, 0.f};
@@ -304,7 +307,7 @@ __global__ __launch_bounds__(512) void kv8_combine_kernel(KvArgs a, AttnArgs t) 
     }
   }
   if (PAIRS * part + item / L >= tile.pairs) return;
-  store_out(t, r, h * D + d, acc, over_sum(l), gate);
+  store_out(t, r, h * D + d, acc, l, sees, gate);
 }
 
 namespace {

@@ -53,7 +53,7 @@ __global__ __launch_bounds__(512) void kv8_attention_wide_kernel(KvArgs a, AttnA
   __shared__ __attribute__((aligned(1024))) char lds[8 * kBytes];
   static_assert(8 * (DT / 2 * 4) * 64 * 16 <= sizeof(lds), "the halves' exchange fits the pages");
   __shared__ __attribute__((aligned(1024))) float scales[4][256];  // of the pages: K's 4, V's 4 (a DMA's room)
-  __shared__ f4 meet[8 * 32];                                      // largest score, sum, V scale of each wave's pairs
+  __shared__ f4 meet[8 * 32];  // largest score, sum, V reference of each wave's pairs, and whether they see anything
   __shared__ Deal<RUNS ? kKvWideSlots : 0> deal;
   __shared__ uint32_t seen_most[8];
   const uint32_t kvh = blockIdx.x % a.kv_heads, run = blockIdx.x / a.kv_heads;
@@ -287,7 +287,7 @@ __global__ __launch_bounds__(512) void kv8_attention_wide_kernel(KvArgs a, AttnA
     // piece i of lane x: the swizzle spreads one pair's pieces over the banks
     auto piece = [](uint32_t of, uint32_t i, uint32_t x) { return (of * kPer + i) * 64 + (x ^ i); };
     l = sum_halves(l);
-    if (f == 0) meet[wave * 32 + r] = f4{m, l, vref, 0.f};
+    if (f == 0) meet[wave * 32 + r] = f4{m, l, vref, seen ? 1.f : 0.f};
 #pragma unroll
     for (int i = 0; i < (int)kPer; ++i) {
       const f16v& v = o[DT / 2 + i / 4];
@@ -314,7 +314,7 @@ __global__ __launch_bounds__(512) void kv8_attention_wide_kernel(KvArgs a, AttnA
       const float wm = state_weight(m, top), wo = state_weight(other[0], top);
       // (a NaN sum stays: a state without a score has weight 0 and, but for NaN, the sum 0)
       const float lt = (m == -INFINITY ? l : l * wm) + (other[0] == -INFINITY ? other[1] : other[1] * wo);
-      const float factor = whole ? over_sum(lt) : 1.0f;
+      const float factor = !whole ? 1.0f : seen ? 1.0f / lt : 0.f;
       const float fm = wm * vref * factor, fo = wo * other[2] * factor;
 #pragma unroll
       for (int i = 0; i < (int)kPer; ++i) {
@@ -341,8 +341,10 @@ __global__ __launch_bounds__(512) void kv8_attention_wide_kernel(KvArgs a, AttnA
       if (pair >= tile.pairs) continue;
       if (whole) {
         if (RUNS && t.gate) read_gate(k, gate);
+        f4 &g0 = gate[RUNS ? 0 : 2 * k], &g1 = gate[RUNS ? 1 : 2 * k + 1];
+        if (t.gate && meet[wave * 32 + pair % 32][3] == 0.f) g0 = g1 = f4{0.f, 0.f, 0.f, 0.f};
         pair_at(t, tile, kvh, pair, row, head);
-        store_out8(t, row, head * D + d, v0, v1, gate[RUNS ? 0 : 2 * k], gate[RUNS ? 1 : 2 * k + 1]);
+        store_out8(t, row, head * D + d, v0, v1, g0, g1);
       } else {
         float* const to = state_of<D, kKvWideTile>(t, kvh, run, u == first_u ? 0 : 1) + pair * D + d;
         *(f4*)to = v0;

@@ -623,9 +623,9 @@ int dh_kv8_append(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, uint32_t
 
 /* y[r, h] = softmax_t(scale * q[r, h] . K[t, g]) . V[t, g] (x sigmoid(gate[r, h])),
  * over tokens t = 0 ..= qpos[r] of row r's sequence, kv head g = h / (heads /
- * kv_heads); a row without a position sees no token and its y is zero. q fp16
- * [rows, heads * head_dim] row stride ldq, y fp16 row stride ldy, gate (may be
- * NULL) fp32 row stride ldg; scores and softmax fp32; the products of a weight
+ * kv_heads); a row without a position sees no token and its y is zero,
+ * whatever its q and gate hold. q fp16 [rows, heads * head_dim] row stride ldq,
+ * y fp16 row stride ldy, gate (may be NULL) fp32 row stride ldg; scores and softmax fp32; the products of a weight
  * and its block's V scale, relative to the largest that the row meets, are
  * rounded to fp16 as the operand of their product with V's codes. max_tokens:
  * how many tokens the longest row sees, for the launch's division of long

@@ -1001,3 +1001,60 @@ def test_warm_up_covers_every_operator_of_the_cache(gpu, stream):
         kernels.kv8.copy_pages(stream, t.cache, (u32([0]), 0), (u32([1]), 0), 1)
         sync()
     assert kernels.gemm.fast_pipelines() == n
+
+
+# (rows, heads, kv heads, head dims, tokens): tiles of 16, of 16 in runs, of 128, of 128 in runs
+KINDS = [(5, 8, 2, 128, 100), (9, 4, 1, 256, 70), (40, 6, 3, 64, 90), (5, 8, 2, 128, 4000), (7, 12, 4, 256, 3000),
+         (3, 2, 1, 64, 6000), (330, 32, 4, 128, 400), (260, 40, 4, 256, 300), (650, 64, 4, 64, 700),
+         (120, 12, 2, 128, 5000), (130, 16, 4, 256, 4200)]
+
+
+def raw_attention(kernels, stream, t, heads, q, gate=None, scale=None):
+    wide = heads * t.dim
+    y, qd, gd = full((t.rows, wide), np.float16, 7), to_dev(q), to_dev(gate) if gate is not None else None
+    most = int((t.qpos.astype(np.uint32) + np.uint32(1)).max())
+    kernels.kv8.attention(stream, t.cache, t.layer, t.batch, (qd, 0), wide, heads, t.dim ** -0.5 if scale is None else scale,
+                          (y, 0), wide, most, (gd, 0) if gate is not None else None, wide)
+    sync()
+    return to_host(y).reshape(t.rows, heads, t.dim)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("rows,heads,kv,dim,n", KINDS)
+def test_attention_of_padding_rows_is_zero_whatever_they_hold(gpu, kernels, stream, rows, heads, kv, dim, n, fmt):
+    """Rows without a position, as a padded batch has them: their queries and gates are NaN, infinite or the type's lowest,
+    their outputs zero, and the other rows keep the bits that they have beside clean ones."""
+    t = Setup(kv, dim, fmt, [n], [rows], layers=1, layer=0, seed=n, behind=0)
+    t.fill([n])
+    t.qpos[1:rows:3] = NONE
+    t.device()
+    q = t.rng.standard_normal((rows, heads * dim)).astype(np.float16)
+    gate = t.rng.standard_normal((rows, heads * dim)).astype(np.float32)
+    clean = raw_attention(kernels, stream, t, heads, q, gate)
+    for i, (a, b) in enumerate([(np.nan, np.nan), (np.inf, np.inf), (-np.inf, -np.inf), (-65504.0, -3.4e38)]):
+        q[1 + 3 * i:rows:12], gate[1 + 3 * i:rows:12] = a, b
+    got = raw_attention(kernels, stream, t, heads, q, gate)
+    none = t.qpos == NONE
+    assert (got[none] == 0).all() and (clean[none] == 0).all()
+    assert np.isfinite(clean.astype(np.float32)).all() and np.array_equal(got[~none], clean[~none])
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("rows,heads,kv,dim,n", KINDS)
+def test_attention_of_queries_that_are_not_finite_is_nan(gpu, kernels, stream, rows, heads, kv, dim, n, fmt):
+    """An infinite or NaN element of a query makes its scores infinite, of either sign, or NaN; the softmax of any of them is
+    NaN, also where every score is -infinity. The other rows and heads keep their bits."""
+    t = Setup(kv, dim, fmt, [n], [rows], layers=1, layer=0, seed=n + 1, behind=0)
+    k = t.rng.standard_normal((n, kv, dim)).astype(np.float32)
+    k[:, :, 5] = np.abs(k[:, :, 5]) + 0.5  # a query that is -inf there has no other score than -inf
+    t.host[0].append(t.table, np.array([0, n]), np.arange(n), k, t.rng.standard_normal(k.shape).astype(np.float32))
+    t.device()
+    q = t.rng.standard_normal((rows, heads, dim)).astype(np.float16)
+    clean = raw_attention(kernels, stream, t, heads, q.reshape(rows, -1))
+    bad = np.zeros((rows, heads), bool)
+    for i, v in enumerate((-np.inf, np.inf, np.nan)):
+        q[i::5, i % heads, 5] = v
+        bad[i::5, i % heads] = True
+    got = raw_attention(kernels, stream, t, heads, q.reshape(rows, -1))
+    assert np.isnan(got[bad].astype(np.float32)).all()
+    assert np.isfinite(clean.astype(np.float32)).all() and np.array_equal(got[~bad], clean[~bad])
