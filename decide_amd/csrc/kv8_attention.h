@@ -257,6 +257,21 @@ __device__ __forceinline__ float state_weight(float m, float top) {
   return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
 }
 
+// Masks the scores of a block of which a pair sees `mine` tokens. They are scaled in the exponent, as where all is seen, so
+// that a mask that is there for another pair of the tile rounds nothing twice: `unit` is what they are yet to be multiplied
+// by. A factor that is 0 or NaN goes in beforehand: it would make NaN of the masked ones' -infinity.
+template <typename V>
+__device__ __forceinline__ void mask_scores(V& s, float cs, uint32_t mine, float& unit) {
+  const bool early = mine != 0 && !(cs > 0.f);
+  if (__any(early)) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] *= early ? cs : 1.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = i < (int)mine ? s[i] : -INFINITY;
+  unit = mine != 0 && cs > 0.f ? cs : 1.0f;
+}
+
 // V's scales differ from block to block, so what a pair rounds to fp16 is the product of a token's weight and its block's
 // scale, relative to `vref`: at least the largest block's share (its largest weight times its scale) over 2^8 among the
 // blocks that this pair sees, and at most the largest. So the products stay at most 2^8, and each is off by 2^-11 of

@@ -127,7 +127,7 @@ __global__ __launch_bounds__(512) void kv8_attention_kernel(KvArgs a, AttnArgs t
       }
       float sv[16];
       const float cs = c * (bad ? NAN : ks0);
-      float unit = cs;  // scores are sv * unit, or sv where a mask has scaled them
+      float unit = cs;  // scores are sv * unit
 #pragma unroll
       for (int i = 0; i < 16; ++i) sv[i] = st[i / 4][i % 4];
       float vs = vs0;
@@ -135,9 +135,7 @@ __global__ __launch_bounds__(512) void kv8_attention_kernel(KvArgs a, AttnArgs t
       const uint32_t tok0 = b * kKvPage + 16 * g;  // below 2^32, as seen is
       if (b * kKvPage + (kKvPage - 1) >= least) {  // some pair does not see all of the page
         const uint32_t mine = seen > tok0 ? min(seen - tok0, 16u) : 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sv[i] = i < (int)mine ? sv[i] * cs : -INFINITY;
-        unit = 1.0f;
+        mask_scores(sv, cs, mine, unit);
         blind = mine == 0;
         // What none sees may be anything, and so may what stands in for a bad page, for those that do not see it.
         if (tok0 >= most || bad) vs = 0.f;

@@ -214,14 +214,12 @@ __global__ __launch_bounds__(512) void kv8_attention_wide_kernel(KvArgs a, AttnA
         const float ks = scales[at][2 * T + f];
         float vs = scales[at][4 + 2 * T + f];
         const float cs = c * (bad ? NAN : ks);
-        float unit = cs;  // scores are st * unit, or st where a mask has scaled them
+        float unit = cs;  // scores are st * unit
         bool blind = false;
         if (b * kKvPage + 32 * T + 31 >= wleast) {  // some pair does not see all of the half
           const uint32_t tok0 = b * kKvPage + 16 * (2 * T + f);  // below 2^32, as seen is
           const uint32_t mine = seen > tok0 ? min(seen - tok0, 16u) : 0;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) st[i] = i < (int)mine ? st[i] * cs : -INFINITY;
-          unit = 1.0f;
+          mask_scores(st, cs, mine, unit);
           blind = mine == 0;
           if (tok0 >= most || bad) vs = 0.f;
         }

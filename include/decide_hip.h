@@ -638,10 +638,11 @@ int dh_kv8_append(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, uint32_t
  * ldq % 8 == 0, ldy % 4 == 0, ldg % 4 == 0; q and gate 16-byte, y 8-byte
  * aligned. Long sequences are divided across workgroups and merged through the
  * context's forward-kernel workspace (dh_kv8_attention_ws; an eager call of
- * the same sizes also grows it). The cuts depend on the call's sizes and on how
- * many pages its rows see, found on the device: a row's bits depend on its own
- * query, position and pages and, where its sequence is cut, on the other rows
- * of the call (rounding only). The same call gives the same bits. */
+ * the same sizes also grows it). The kernel and the cuts depend on the call's
+ * sizes, the cuts also on how many pages its rows see, found on the device. For
+ * given sizes a row's bits depend on its own query, gate, position and pages
+ * and, where the call's sequences are cut, on the positions of the other rows
+ * (rounding only). The same call gives the same bits. */
 int dh_kv8_attention(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, uint32_t layer, const dh_kv8_batch* batch,
                      const uint16_t* q, uint32_t ldq, uint32_t heads, float scale, const float* gate, uint32_t ldg,
                      uint16_t* y, uint32_t ldy, uint32_t max_tokens);

@@ -1058,3 +1058,28 @@ def test_attention_of_queries_that_are_not_finite_is_nan(gpu, kernels, stream, r
     got = raw_attention(kernels, stream, t, heads, q.reshape(rows, -1))
     assert np.isnan(got[bad].astype(np.float32)).all()
     assert np.isfinite(clean.astype(np.float32)).all() and np.array_equal(got[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("rows,heads,kv,dim,n", [k for k in KINDS if k[4] < 1000] + [(16, 16, 4, 256, 1000), (700, 32, 4, 128, 1400)])
+def test_the_bits_of_a_row_that_is_not_cut_are_its_own(gpu, kernels, stream, rows, heads, kv, dim, n, fmt):
+    """Where no sequence is divided, a row's bits depend on its own query, position and pages: every other row moves (to the
+    start, behind a large block, out of sight), and the rest keep theirs."""
+    t = Setup(kv, dim, fmt, [n], [rows], layers=1, layer=0, seed=n + 2, behind=0)
+    k, v = (t.rng.standard_normal((n, kv, dim)).astype(np.float32) for _ in range(2))
+    v[n // 2:n // 2 + 9] *= np.float32(300.0)
+    t.host[0].append(t.table, np.array([0, n]), np.arange(n), k, v)
+    t.qpos[:] = t.rng.integers(0, n, rows)
+    t.qpos[0::2] = np.sort(t.qpos[0::2])
+    q = t.rng.standard_normal((rows, heads * dim)).astype(np.float16)
+    first, stay = None, np.arange(rows) % 2 == 0
+    for move in (None, 0, n - 1, NONE, 17):
+        if move is not None:
+            t.qpos[~stay] = move
+        t.device()
+        qq = q.copy()
+        if move == 17:
+            qq[~stay] = np.inf
+        got = raw_attention(kernels, stream, t, heads, qq)
+        first = got if first is None else first
+        assert np.array_equal(got[stay], first[stay]), (move, np.argwhere((got != first).any((1, 2)) & stay).ravel()[:9])
