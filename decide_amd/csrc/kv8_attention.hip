@@ -332,6 +332,8 @@ uint64_t run_bytes(bool wide, uint64_t runs, uint64_t slots, uint32_t kv_heads, 
 }
 }  // namespace
 
+constexpr uint32_t kMinRun = 8;
+
 KvAttnPlan kv8_attention_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
                               uint32_t ld_table, uint32_t max_tokens, uint32_t cus) {
   KvAttnPlan p;
@@ -348,10 +350,11 @@ KvAttnPlan kv8_attention_plan(uint32_t rows, uint32_t seqs, uint32_t heads, uint
   // tokens 10.6 against 10.2, 8,000 11.1 against 19.8. 1,500 rows in runs: 341 against 95. Wide tiles of 4 heads of 256:
   // 256 rows behind 7,744 tokens 72 against 212, 1,000 rows of 8,000 169 against 214, 1,000 causal rows 95 against 45.
   if (pages < least_pages(p.wide, head_dim) || (p.wide ? slots * kv_heads : full) >= cus ||
-      (p.wide && head_dim == 64) || slots > (p.wide ? kKvWideSlots : kKvMaxSlots) || slots * (ld_table + 1ull) > UINT32_MAX)
+      (p.wide && head_dim == 64) || slots > (p.wide ? kKvWideSlots : kKvMaxSlots) ||
+      slots * (ld_table + 1ull) > UINT32_MAX - std::max(cus, kMinRun))  // all pages, rounded up to whole runs, in 32 bits
     return p;
   p.runs = std::max<uint32_t>(1, cus / kv_heads);
-  p.min_run = p.wide ? 4 : 8;  // a page for each wave; fewer, and the states' share grows
+  p.min_run = p.wide ? 4 : kMinRun;  // a page for each wave; fewer, and the states' share grows
   p.ws_bytes = run_bytes(p.wide, p.runs, p.slots, kv_heads, head_dim);
   return p;
 }

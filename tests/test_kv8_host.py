@@ -329,3 +329,20 @@ def test_the_reserved_workspace_covers_the_call_and_every_smaller_one(dim, cus):
                     assert p.ws_bytes <= held, (kv, group, rows, tokens, n, g, t, seqs, p.wide, p.ws_bytes, held)
                     sizes, runs, wide = sizes + 1, runs + (p.runs > 0), wide + (p.wide and p.runs > 0)
     assert runs > sizes // 20 and (wide > 50 or dim == 64)  # the sweep meets what it is for
+
+
+@pytest.mark.parametrize("cus", [256, 304, 64])
+def test_runs_whose_pages_round_up_past_32_bits_are_not_taken(cus):
+    """The device counts the tiles' pages in 32 bits (at most one more than the table has, each), rounds their number up to
+    whole runs and adds a run's share to where it starts."""
+    plan, _ = _attention_sizes()
+    end = 1 << 32
+    for rows in (1, 63, 65, 1900):
+        slots = rows + rows // 16
+        for ld_table in (end // slots - 1 - i for i in (0, 1, 2, 5, 100, 300, 1000)):
+            p = plan(rows, rows, 4, 4, 64, ld_table, 8192, cus)
+            pages = slots * (ld_table + 1)
+            assert p.slots == slots and (p.runs or pages > end - 1000)
+            if p.runs:
+                share = max(-(-pages // p.runs), p.min_run)
+                assert pages + p.runs - 1 < end and -(-pages // share) * share < end
