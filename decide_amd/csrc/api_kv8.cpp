@@ -173,7 +173,7 @@ int dh_kv8_append(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, uint32_t
   if (batch->rows && batch->seqs && (!k || !v)) return fail(DH_EINVAL, "kv8_append: null pointer");
   if (batch->rows && batch->seqs) mark(ctx, kKidKv8Append);
   return hip_status(dh::launch_kv8_append(kv_args(cache, layer, batch), cache->head_dim, cache->format == DH_KV8_INT8, k,
-                                          ldk, v, ldv, dtype, rope_args(rope), (hipStream_t)stream),
+                                          ldk, v, ldv, dtype, rope_args(rope), ctx->cus, (hipStream_t)stream),
                     "kv8_append");
 }
 
@@ -211,7 +211,7 @@ int dh_kv8_attention(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, uint3
   mark(ctx, kKidKv8Attn);
   return hip_status(dh::launch_kv8_attention(kv_args(cache, layer, batch), cache->head_dim,
                                              cache->format == DH_KV8_INT8, (const _Float16*)q, ldq, heads, scale, gate,
-                                             ldg, (_Float16*)y, ldy, aux, plan, (hipStream_t)stream),
+                                             ldg, (_Float16*)y, ldy, aux, plan, ctx->cus, (hipStream_t)stream),
                     "kv8_attention");
 }
 
@@ -278,7 +278,7 @@ int kv8_warm(dh_ctx* ctx, hipStream_t s, void* mem) {
     for (const dh::KvAttnPlan& plan : {dh::KvAttnPlan{1, 1, 8, false, 0}, dh::KvAttnPlan{1, 0, 0, true, 0}})
       if (rc == DH_OK)
         rc = hip_status(dh::launch_kv8_attention(kv_args(&cache, 0, &batch), 64, false, (const _Float16*)x, 64, 1, 1.f,
-                                                 nullptr, 0, (_Float16*)y, 64, (float*)(base + 49152), plan, s),
+                                                 nullptr, 0, (_Float16*)y, 64, (float*)(base + 49152), plan, ctx->cus, s),
                         "kv8_attention");
   }
   if (rc == DH_OK) rc = dh_kv8_copy_pages(ctx, s, &cache, u, u, 1);  // page 0 onto itself

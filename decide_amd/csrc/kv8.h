@@ -32,9 +32,9 @@ struct KvArgs {
 // elements of x and y: 0 fp16, 1 bf16, 2 fp32
 hipError_t launch_rope(const void* x, uint32_t ldx, uint32_t x_dtype, void* y, uint32_t ldy, uint32_t y_dtype,
                        const uint32_t* pos, uint32_t rows, uint32_t heads, const RopeArgs& rope, hipStream_t s);
-// rope.inv_freq null: keys are coded as they are
+// rope.inv_freq null: keys are coded as they are; cus: compute units of the device
 hipError_t launch_kv8_append(const KvArgs& a, uint32_t head_dim, bool int8, const void* k, uint32_t ldk, const void* v,
-                             uint32_t ldv, uint32_t dtype, const RopeArgs& rope, hipStream_t s);
+                             uint32_t ldv, uint32_t dtype, const RopeArgs& rope, uint32_t cus, hipStream_t s);
 hipError_t launch_kv8_copy_pages(uint8_t* pool, uint64_t page_bytes, uint32_t pages, uint32_t layers,
                                  const uint32_t* src, const uint32_t* dst, uint32_t n, hipStream_t s);
 
@@ -59,6 +59,6 @@ uint64_t kv8_attention_ws_bytes(uint32_t rows, uint32_t heads, uint32_t kv_heads
                                 uint32_t cus);
 hipError_t launch_kv8_attention(const KvArgs& a, uint32_t head_dim, bool int8, const _Float16* q, uint32_t ldq,
                                 uint32_t heads, float scale, const float* gate, uint32_t ldg, _Float16* y,
-                                uint32_t ldy, float* ws, const KvAttnPlan& plan, hipStream_t s);
+                                uint32_t ldy, float* ws, const KvAttnPlan& plan, uint32_t cus, hipStream_t s);
 
 }  // namespace dh

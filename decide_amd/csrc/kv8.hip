@@ -531,12 +531,12 @@ hipError_t launch_rope(const void* x, uint32_t ldx, uint32_t x_dtype, void* y, u
 namespace {
 template <typename T, bool INT8>
 void append_dim(const KvArgs& a, uint32_t head_dim, const void* k, uint32_t ldk, const void* v, uint32_t ldv,
-                const RopeArgs& p, hipStream_t s) {
+                const RopeArgs& p, uint32_t cus, hipStream_t s) {
   // A workgroup takes one head after another where there would be more of them than run at once (four a CU):
   // 385 blocks of 8 heads 21.4 us with one head each, 17.0 with four, 15.9 with eight; 146 blocks of 4 heads 14.0 with one,
   // 15.9 with two.
   const uint64_t single = ((uint64_t)a.rows / kKvBlock + a.seqs) * 2 * a.kv_heads;
-  const uint32_t at_once = (uint32_t)std::min<uint64_t>(a.kv_heads, std::max<uint64_t>(1, single / 1024));
+  const uint32_t at_once = (uint32_t)std::min<uint64_t>(a.kv_heads, std::max<uint64_t>(1, single / (4ull * cus)));
   const dim3 grid(a.rows / kKvBlock + 2 * a.seqs, 2 * ((a.kv_heads + at_once - 1) / at_once));
   const size_t lds = p.inv_freq ? (size_t)4 * 4 * (p.rot / 2) * 2 * sizeof(double) : 0;
   if (head_dim == 64)
@@ -551,23 +551,23 @@ void append_dim(const KvArgs& a, uint32_t head_dim, const void* k, uint32_t ldk,
 }
 template <typename T>
 void append_format(const KvArgs& a, uint32_t head_dim, bool int8, const void* k, uint32_t ldk, const void* v,
-                   uint32_t ldv, const RopeArgs& p, hipStream_t s) {
+                   uint32_t ldv, const RopeArgs& p, uint32_t cus, hipStream_t s) {
   if (int8)
-    append_dim<T, true>(a, head_dim, k, ldk, v, ldv, p, s);
+    append_dim<T, true>(a, head_dim, k, ldk, v, ldv, p, cus, s);
   else
-    append_dim<T, false>(a, head_dim, k, ldk, v, ldv, p, s);
+    append_dim<T, false>(a, head_dim, k, ldk, v, ldv, p, cus, s);
 }
 }  // namespace
 
 hipError_t launch_kv8_append(const KvArgs& a, uint32_t head_dim, bool int8, const void* k, uint32_t ldk, const void* v,
-                             uint32_t ldv, uint32_t dtype, const RopeArgs& p, hipStream_t s) {
+                             uint32_t ldv, uint32_t dtype, const RopeArgs& p, uint32_t cus, hipStream_t s) {
   if (a.rows == 0 || a.seqs == 0) return hipSuccess;
   if (dtype == 0)
-    append_format<Half>(a, head_dim, int8, k, ldk, v, ldv, p, s);
+    append_format<Half>(a, head_dim, int8, k, ldk, v, ldv, p, cus, s);
   else if (dtype == 1)
-    append_format<Bf16>(a, head_dim, int8, k, ldk, v, ldv, p, s);
+    append_format<Bf16>(a, head_dim, int8, k, ldk, v, ldv, p, cus, s);
   else
-    append_format<float>(a, head_dim, int8, k, ldk, v, ldv, p, s);
+    append_format<float>(a, head_dim, int8, k, ldk, v, ldv, p, cus, s);
   return hipGetLastError();
 }
 

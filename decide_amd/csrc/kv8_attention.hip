@@ -381,7 +381,7 @@ void narrow_kernels(const KvArgs& a, const AttnArgs& t, bool int8, hipStream_t s
   int8 ? with(std::true_type{}) : with(std::false_type{});
 }
 template <int D>
-hipError_t attention_of(const KvArgs& a, const AttnArgs& t, bool int8, bool wide, hipStream_t s) {
+hipError_t attention_of(const KvArgs& a, const AttnArgs& t, bool int8, bool wide, uint32_t cus, hipStream_t s) {
   if (!wide) narrow_kernels<D>(a, t, int8, s);
   const hipError_t e = wide ? launch_kv8_wide(a, t, D, int8, s) : hipGetLastError();
   if (!t.runs || e != hipSuccess) return e;
@@ -390,7 +390,7 @@ hipError_t attention_of(const KvArgs& a, const AttnArgs& t, bool int8, bool wide
     if constexpr (D != 64)
       hipLaunchKernelGGL((kv8_combine_kernel<D, kKvWideTile, kPairs>),
                          dim3(a.kv_heads * t.slots * (kKvWideTile / kPairs)), dim3(512), 0, s, a, t);
-  } else if (a.kv_heads * t.slots * (kKvTile / kPairs) <= 1024)  // (four workgroups a CU)
+  } else if (a.kv_heads * t.slots * (kKvTile / kPairs) <= 4 * cus)
     hipLaunchKernelGGL((kv8_combine_kernel<D, kKvTile, kPairs>), dim3(a.kv_heads * t.slots * (kKvTile / kPairs)),
                        dim3(512), 0, s, a, t);
   else
@@ -402,15 +402,15 @@ hipError_t attention_of(const KvArgs& a, const AttnArgs& t, bool int8, bool wide
 
 hipError_t launch_kv8_attention(const KvArgs& a, uint32_t head_dim, bool int8, const _Float16* q, uint32_t ldq,
                                 uint32_t heads, float scale, const float* gate, uint32_t ldg, _Float16* y,
-                                uint32_t ldy, float* ws, const KvAttnPlan& p, hipStream_t s) {
+                                uint32_t ldy, float* ws, const KvAttnPlan& p, uint32_t cus, hipStream_t s) {
   if (a.rows == 0 || a.seqs == 0) return hipSuccess;
   if (p.runs && (!ws || p.min_run == 0 || (p.wide && head_dim == 64) || p.slots > (p.wide ? kKvWideSlots : kKvMaxSlots))) return hipErrorInvalidValue;
   const uint32_t group = heads / a.kv_heads;
   const AttnArgs t{q,     gate,    y,      ws,        ldq,  ldg, ldy, heads, group, ((1u << 21) + group - 1) / group,
                    p.slots, p.runs, p.min_run, scale};
-  if (head_dim == 64) return attention_of<64>(a, t, int8, p.wide, s);
-  if (head_dim == 128) return attention_of<128>(a, t, int8, p.wide, s);
-  return attention_of<256>(a, t, int8, p.wide, s);
+  if (head_dim == 64) return attention_of<64>(a, t, int8, p.wide, cus, s);
+  if (head_dim == 128) return attention_of<128>(a, t, int8, p.wide, cus, s);
+  return attention_of<256>(a, t, int8, p.wide, cus, s);
 }
 
 }  // namespace dh
