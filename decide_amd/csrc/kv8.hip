@@ -7,7 +7,10 @@
 //   append  codes K and V rows into pages, a workgroup a block (16 tokens of one head, K or V).
 //   copy    moves whole pages, 16 bytes a lane.
 //
-// All three are bound by memory: each value is read once and written once.
+// Each value is read once and written once. Rotations of many rows and copies run at 90 % of a large copy's rate; the append
+// does not: 2,307 rows of 4 heads of 256 take 14.4 us where their bytes take 4.4. Its workgroups read the row range, the
+// position, the page and the started block one after another, each head's form the same angles in 64 bits, and V is read one
+// element a lane; how much each of these costs was not measured apart.
 #include <algorithm>
 #include <cmath>
 

@@ -275,8 +275,9 @@ __device__ __forceinline__ void mask_scores(V& s, float cs, uint32_t mine, float
 // V's scales differ from block to block, so what a pair rounds to fp16 is the product of a token's weight and its block's
 // scale, relative to `vref`: at least the largest block's share (its largest weight times its scale) over 2^8 among the
 // blocks that this pair sees, and at most the largest. So the products stay at most 2^8, and each is off by 2^-11 of
-// itself or 2^-25 of the largest share, whatever scales unseen blocks or those of next to no weight have. Relative to the
-// largest scale alone, a block of values 2^20 larger behind a row's position took 5 % of that row.
+// itself or 2^-25 of the largest share, whatever scales unseen blocks or those of next to no weight have. (A block that is
+// seen in part counts with its whole scale, which its seen tokens are coded in: a code's half step is 2^-10 of it at least.)
+// Relative to the largest scale alone, a block of values 2^20 larger behind a row's position took 5 % of that row.
 constexpr float kNoScale = 0x1p-100f;   // no block's scale is smaller
 constexpr float kMostScale = 0x1p126f;  // vref's, and a ratio's, largest: the reciprocal and the products stay finite
 __device__ __forceinline__ float block_share(float top, float m, float vs) {

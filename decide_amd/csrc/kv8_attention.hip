@@ -17,7 +17,7 @@
 //     end one tile and begin another. A tile that lies in several runs leaves a state (largest score, sum, O) per run, and
 //     kv8_combine_kernel merges them in order. With pieces of a fixed length instead, sized by the longest sequence, 64
 //     sequences of up to 8,192 tokens made 2,560 workgroups, 2,100 of them empty, and took 77 us against 52.
-//   * Long sequences: bound by HBM (one row behind 131,072 tokens, 8 heads of 128, 51 us: 5.3 TB/s). Short ones: by the
+//   * Long sequences: bound by HBM (one row behind 131,072 tokens, 8 heads of 128, 52 us: 5.1 TB/s). Short ones: by the
 //     chain of reads row range, position, Q, page number, page, and the waves' merge (603 tokens 12 us, any number of heads).
 #include <algorithm>
 

@@ -8,10 +8,11 @@
 //     of half T gets the 16 scores of pair r and block 2 T + f, which are P^T V's operand as they are.
 //   * 16-byte chunk x of K's token t lies at chunk x ^ key(t), of V's dim d at x ^ (d / 2 % 4), so that eight lanes
 //     that read at once read 128 different bytes' banks.
-//   * Bound by the issue of vector instructions: two waves of a SIMD have 340 each a page, 4 clocks apart at best (one wave
-//     alone issues every 6 to 7), and the matrix cores are busy for 2,048 clocks of a page's 4,100. The halves are kept half a
-//     page apart, and the one at its products has priority. With four waves, each taking both halves, 37 pages took 96 us
-//     against 76; with one barrier for all every two pages 82.
+//   * A page takes 2.1 to 2.5 us with every CU busy (2,040 rows behind 8,192 tokens against 4,096). The two waves of a SIMD
+//     have 375 vector instructions each a page (35 more where a row is masked), 4 clocks apart at best and 16 for the 20
+//     transcendental ones, 3,500 clocks together, beside 2,048 of products: at 2.4 GHz 1.45 and 0.85 us, overlapped in
+//     part. What the rest is was not taken apart. The halves are kept half a page apart, so that one is at its products
+//     while the other is at its softmax, and the one at its products has priority.
 //   * The two halves meet once, at a tile's end, through LDS: each takes half of the dims.
 #include "kv8_attention.h"
 
@@ -194,7 +195,7 @@ __global__ __launch_bounds__(512) void kv8_attention_wide_kernel(KvArgs a, AttnA
         const char* const kb = lds + at * 2 * kBytes + tok * D;
         uint32_t sw = (f ^ k_key<D>(tok)) * 16;  // chunk 2 x + f of the token lies at byte 32 x ^ sw
         asm volatile("" : "+v"(sw));             // formed here: hoisted addresses would spill
-        __builtin_amdgcn_s_setprio(1);  // the wave at its products goes first: 37 pages 84 us against 76
+        __builtin_amdgcn_s_setprio(1);  // the wave at its products goes first: 2,307 causal rows 101 us against 93
         f16v st;
 #pragma unroll
         for (int e = 0; e < 16; ++e) st[e] = 0.f;

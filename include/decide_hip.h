@@ -654,7 +654,8 @@ int dh_kv8_attention_ws(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, ui
 
 /* Copies page src[i] to page dst[i] in every layer, i < n (device arrays):
  * what dh_pages_resize and dh_pages_compact ask for. A pair with an id not
- * below cache->pages is left out. No dst may be another pair's src or dst. */
+ * below cache->pages is left out. No dst may be another pair's src or dst.
+ * n <= cache->pages, pairs that are left out among them. */
 int dh_kv8_copy_pages(dh_ctx* ctx, void* stream, const dh_kv8_cache* cache, const uint32_t* src, const uint32_t* dst,
                       uint32_t n);
 
