@@ -287,6 +287,10 @@ __device__ __forceinline__ float block_share(float top, float m, float vs) {
 __device__ __forceinline__ bool moves(float bm, float m, float vm, float vref) {
   return bm > m + kLazy || vm > 256.0f * vref;
 }
+// (blocks that were never written, with scales of zero, leave it where it was)
+__device__ __forceinline__ float next_reference(float vold, float share) {
+  return fminf(fmaxf(fmaxf(vold, share), kNoScale), kMostScale);
+}
 __device__ __forceinline__ float scale_ratio(float vs, float vref) {
   const float r = vs * __builtin_amdgcn_rcpf(vref);  // off by 2^-23 at most
   return r > kMostScale ? kMostScale : r;  // (where weights vanish; a NaN scale stays)

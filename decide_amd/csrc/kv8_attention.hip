@@ -161,7 +161,7 @@ __global__ __launch_bounds__(512) void kv8_attention_kernel(KvArgs a, AttnArgs t
         const bool mine = moves(bm, m, vm, vref);  // a pair's own: the others of the tile keep their bits
         const float mnew = bm > m + kLazy ? bm : m;
         const float alpha = state_weight(m, mnew), vold = alpha * vref;
-        const float vnew = mine ? fminf(fmaxf(vold, share(mnew)), kMostScale) : vref;
+        const float vnew = mine ? next_reference(vold, share(mnew)) : vref;
         const float both = mine ? vold / vnew : 1.0f;
         l *= alpha;
         m = mnew;

@@ -1083,3 +1083,28 @@ def test_the_bits_of_a_row_that_is_not_cut_are_its_own(gpu, kernels, stream, row
         got = raw_attention(kernels, stream, t, heads, qq)
         first = got if first is None else first
         assert np.array_equal(got[stay], first[stay]), (move, np.argwhere((got != first).any((1, 2)) & stay).ravel()[:9])
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("rows,heads,kv,dim,n", KINDS)
+def test_attention_over_a_zeroed_pool_is_zero(gpu, kernels, stream, rows, heads, kv, dim, n, fmt):
+    """Scales of zero, as a pool has them that nothing was written to (a program's dry run): every value is zero, and so is
+    every output; written tokens behind such blocks come out as if those held zeros."""
+    t = Setup(kv, dim, fmt, [n], [rows], layers=1, layer=0, seed=n + 3, behind=0, fill=0)
+    q = t.rng.standard_normal((rows, heads * dim)).astype(np.float16)
+    gate = t.rng.standard_normal((rows, heads * dim)).astype(np.float32)
+    got = raw_attention(kernels, stream, t.device(), heads, q, gate)
+    assert (got == 0).all()
+    t.fill([n])
+    want = t.host[0].s.copy()
+    pages = t.table[0, :2]
+    t.host[0].s[pages] = 0.0
+    zeros = raw_attention(kernels, stream, t.device(), heads, q, gate)
+    t.host[0].s[pages] = want[pages]
+    t.host[0].k, t.host[0].v = t.host[0].k.copy(), t.host[0].v.copy()
+    t.host[0].k[pages] = t.host[0].v[pages] = 0 if fmt == "e4m3" else 128
+    same = raw_attention(kernels, stream, t.device(), heads, q, gate)
+    a, b = zeros.astype(np.float64), same.astype(np.float64)
+    # weights are rounded to fp16 relative to different references: 2^-11 each of what is summed, at most the largest |v|
+    _, v = t.host[0].tokens(t.table[0, :-(-n // ref.PAGE)], n)
+    assert (np.abs(a - b) <= 2.0 ** -9 * np.abs(v).max()).all() and np.isfinite(a).all()
