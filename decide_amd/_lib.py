@@ -89,6 +89,20 @@ class DhRopeSpec(ctypes.Structure):
                 ("layout", c_uint32), ("add_one", c_uint32), ("eps", c_float), ("amp", c_float)]
 
 
+class DhFp8Matrix(ctypes.Structure):
+    """``dh_fp8_matrix`` (include/decide_hip.h)."""
+
+    _fields_ = [("codes", c_void_p), ("scales", c_void_p), ("ld", c_uint32), ("lds", c_uint32)]
+
+
+class DhPackedBatch(ctypes.Structure):
+    """``dh_packed_batch`` (include/decide_hip.h)."""
+
+    _fields_ = [("q0", c_void_p), ("k0", c_void_p), ("seqs", c_uint32), ("q_rows", c_uint32), ("k_rows", c_uint32),
+                ("max_k", c_uint32)]
+
+
+DH_FP8_BLOCK = 128
 DH_KV8_PAGE = 64
 DH_KV8_BLOCK = 16
 DH_KV8_NO_POSITION = 0xFFFFFFFF
@@ -245,6 +259,25 @@ PROTOTYPES = {
         c_int, [c_void_p, c_uint32, POINTER(c_uint64), POINTER(c_uint32), c_uint32, POINTER(c_uint32)]),
     "dh_pages_free": (c_uint32, [c_void_p]),
     "dh_pages_refs": (c_uint32, [c_void_p, c_uint32]),
+    "dh_fp8_quant_rows": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_uint32, c_uint32, c_void_p, c_uint32, c_float, POINTER(DhFp8Matrix), c_uint32,
+         c_uint32],
+    ),
+    "dh_fp8_quant_blocks": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_uint32, c_uint32, POINTER(DhFp8Matrix), c_uint32, c_uint32]),
+    "dh_gemm_fp8": (
+        c_int,
+        [c_void_p, c_void_p, POINTER(DhFp8Matrix), POINTER(DhFp8Matrix), c_void_p, c_uint32, c_uint32, c_uint32, c_uint32,
+         c_uint32],
+    ),
+    "dh_attention_packed": (
+        c_int,
+        [c_void_p, c_void_p, POINTER(DhPackedBatch), c_void_p, c_uint32, c_void_p, c_uint32, c_void_p, c_uint32, c_uint32,
+         c_uint32, c_uint32, c_uint32, c_float, c_void_p, c_uint32, c_void_p, c_uint32],
+    ),
+    "dh_attention_packed_ws": (c_int, [c_void_p, c_void_p, c_uint32, c_uint32, c_uint32, c_uint32, c_uint32]),
+    "dh_gemm_fp8_ws": (c_int, [c_void_p, c_void_p, c_uint32, c_uint32, c_uint32]),
 }
 
 _lib = None

@@ -507,9 +507,9 @@ int dh_warm_up(dh_ctx* ctx, void* stream, uint32_t max_m) {
   void* scratch = nullptr;
   const size_t xb = 16 * 128 * 2, wb = 512 * 64 * 2, yb = 16 * 512 * 4;
   const size_t gemm_bytes = (xb + wb + yb + 127) / 128 * 128;
-  hipError_t e = hipMalloc(&scratch, gemm_bytes + kv8_warm_bytes());
+  hipError_t e = hipMalloc(&scratch, gemm_bytes + kv8_warm_bytes() + fp8_warm_bytes() + 512);
   if (e != hipSuccess) return fail(DH_ENOMEM, "dh_warm_up: %s", hipGetErrorString(e));
-  e = hipMemsetAsync(scratch, 0, gemm_bytes + kv8_warm_bytes(), s);
+  e = hipMemsetAsync(scratch, 0, gemm_bytes + kv8_warm_bytes() + fp8_warm_bytes() + 512, s);
   int rc = hip_status(e, "dh_warm_up memset");
   char* base = (char*)scratch;
   for (int v = 0; v < dh::variant_count() && rc == DH_OK; ++v) {
@@ -528,6 +528,8 @@ int dh_warm_up(dh_ctx* ctx, void* stream, uint32_t max_m) {
     rc = launch_plan(ctx, s, dh::plan_make(0, 2, 8, vi.bn(), 128), base, 128, 8, 128, &mem, 1);
   }
   if (rc == DH_OK) rc = kv8_warm(ctx, s, base + gemm_bytes);
+  if (rc == DH_OK) rc = fp8_warm(ctx, s, base + gemm_bytes + kv8_warm_bytes());
+  if (rc == DH_OK) rc = packed_warm(ctx, s, base + gemm_bytes + kv8_warm_bytes() + fp8_warm_bytes());
   if (rc == DH_OK) {
     e = hipStreamSynchronize(s);
     rc = hip_status(e, "dh_warm_up sync");

@@ -48,7 +48,9 @@ enum : int {
   kKidReduce = kMaxTileVariants, kKidReference, kKidGather32, kKidGather16, kKidHead, kKidNorm, kKidFill,
   kKidConv, kKidConvState, kKidDelta, kKidGNorm, kKidQRope, kKidKVRope, kKidAttn, kKidEmbed, kKidFillAny,
   kKidDeltaChunk, kKidStream, kKidAttnCombine, kKidConvDelta, kKidAddNorm, kKidDeltaBlock,
-  kKidRope, kKidKv8Append, kKidKv8Attn, kKidKv8Combine, kKidKv8Copy, kKidCount
+  kKidRope, kKidKv8Append, kKidKv8Attn, kKidKv8Combine, kKidKv8Copy,
+  kKidFp8Rows, kKidFp8Blocks, kKidFp8Reduce, kKidPacked, kKidPackedMerge, kKidFp8Gemm,  // (and its variants behind it)
+  kKidCount = kKidFp8Gemm + 4
 };
 static_assert(kKidCount <= 64, "kernel ids must fit dh_ctx::used");
 
@@ -78,5 +80,10 @@ int attention_run(dh_ctx* ctx, void* stream, const uint16_t* q, const uint16_t* 
 // loaded by the source file, so the others come with it. `mem` holds kv8_warm_bytes() zeroed bytes.
 size_t kv8_warm_bytes();
 int kv8_warm(dh_ctx* ctx, hipStream_t s, void* mem);
+
+// The same for the 8-bit codes and their product, and for attention over packed sequences (512 zeroed bytes).
+size_t fp8_warm_bytes();
+int fp8_warm(dh_ctx* ctx, hipStream_t s, void* mem);
+int packed_warm(dh_ctx* ctx, hipStream_t s, void* mem);
 
 }  // namespace dh_api

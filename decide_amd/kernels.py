@@ -318,6 +318,15 @@ class Rope:
                                DTYPE_CODES[y_dtype], addr(pos), rows, heads, spec.ref))
 
 
+class PackedBatch:
+    """``dh_packed_batch``: which rows and which keys belong to which sequence. Keeps the buffers alive."""
+
+    def __init__(self, q0: Arg, k0: Arg, seqs: int, q_rows: int, k_rows: int, max_k: int):
+        self.keep = (q0, k0)
+        self.c = _lib.DhPackedBatch(addr(q0), addr(k0), seqs, q_rows, k_rows, max_k)
+        self.ref = ctypes.byref(self.c)
+
+
 class Attn:
     """decide's ``Attn`` (kernels/attn.rs:44-125)."""
 
@@ -329,6 +338,18 @@ class Attn:
                   ldq: int) -> None:
         _call(self.lib.dh_attention(self.ctx.handle, ctypes.c_void_p(stream), addr(q), addr(kc), addr(vc), addr(pq),
                                     addr(qpos), addr(y), rows, ldq))
+
+    def packed(self, stream: int, batch: PackedBatch, q: Arg, ldq: int, k: Arg, ldk: int, v: Arg, ldv: int, dtype: str,
+               heads: int, kv_heads: int, head_dim: int, scale: float, y: Arg, ldy: int, gate: Optional[Arg] = None,
+               ldg: int = 0) -> None:
+        """y = softmax(scale q·kᵀ)·v (⊙ σ(gate)) of packed sequences' rows, causal; decide has only ``attention``'s form."""
+        _call(self.lib.dh_attention_packed(self.ctx.handle, stream, batch.ref, addr(q), ldq, addr(k), ldk, addr(v), ldv,
+                                           DTYPE_CODES[dtype], heads, kv_heads, head_dim, scale,
+                                           None if gate is None else addr(gate), ldg, addr(y), ldy))
+
+    def packed_ws(self, stream: int, q_rows: int, seqs: int, heads: int, kv_heads: int, head_dim: int) -> None:
+        """Sizes ``stream``'s workspace for ``packed`` calls of up to these sizes (before a capture)."""
+        _call(self.lib.dh_attention_packed_ws(self.ctx.handle, stream, q_rows, seqs, heads, kv_heads, head_dim))
 
 
 def kv8_page_bytes(kv_heads: int, head_dim: int) -> int:
@@ -381,6 +402,44 @@ class Kv8:
     def copy_pages(self, stream: int, cache: Kv8Cache, src: Arg, dst: Arg, n: int) -> None:
         """Page src[i] → dst[i] in every layer, i < n (device arrays of page ids)."""
         _call(self.lib.dh_kv8_copy_pages(self.ctx.handle, stream, cache.ref, addr(src), addr(dst), n))
+
+
+class Fp8Matrix:
+    """``dh_fp8_matrix``: e4m3 codes [rows][ld] and their scales' bytes [ceil(columns / 512)][lds][4]. Keeps its buffers
+    alive."""
+
+    def __init__(self, codes: Arg, ld: int, scales: Arg, lds: int):
+        self.keep = (codes, scales)
+        self.c = _lib.DhFp8Matrix(addr(codes), addr(scales), ld, lds)
+        self.ref = ctypes.byref(self.c)
+
+
+class Fp8:
+    """8-bit floating point with a scale for each block of 128 (decide's GEMM path is fp16: kernels/gemm.rs:126-176)."""
+
+    def __init__(self, ctx: Context):
+        self.ctx = ctx
+        self.lib = ctx.lib
+
+    def quant_rows(self, stream: int, x: Arg, ldx: int, dtype: str, out: Fp8Matrix, rows: int, k: int,
+                   norm_w: Optional[Arg] = None, add_one: bool = True, eps: float = 1e-6) -> None:
+        """Codes rows (normed first, with ``norm_w``) with a scale for each row and 128 columns."""
+        _call(self.lib.dh_fp8_quant_rows(self.ctx.handle, stream, addr(x), ldx, DTYPE_CODES[dtype],
+                                         None if norm_w is None else addr(norm_w), 1 if add_one else 0, eps, out.ref,
+                                         rows, k))
+
+    def quant_blocks(self, stream: int, w: Arg, ldw: int, dtype: str, out: Fp8Matrix, n: int, k: int) -> None:
+        """Codes a weight's rows with a scale for each 128 rows and 128 columns."""
+        _call(self.lib.dh_fp8_quant_blocks(self.ctx.handle, stream, addr(w), ldw, DTYPE_CODES[dtype], out.ref, n, k))
+
+    def gemm(self, stream: int, x: Fp8Matrix, w: Fp8Matrix, y: Arg, ldy: int, m: int, n: int, k: int,
+             epi: Epilogue) -> None:
+        """``Y = X · Wᵀ`` of coded rows and a coded weight, then ``epi`` as in ``Gemm.gemm``; fp32 accumulation."""
+        _call(self.lib.dh_gemm_fp8(self.ctx.handle, stream, x.ref, w.ref, addr(y), ldy, m, n, k, int(epi)))
+
+    def gemm_ws(self, stream: int, max_m: int, n: int, k: int) -> None:
+        """Sizes ``stream``'s workspace for ``gemm`` calls of up to ``max_m`` rows (before a capture)."""
+        _call(self.lib.dh_gemm_fp8_ws(self.ctx.handle, stream, max_m, n, k))
 
 
 class Pages:
@@ -464,3 +523,4 @@ class Kernels:
         self.rope = Rope(self.ctx)
         self.attn = Attn(self.ctx)
         self.kv8 = Kv8(self.ctx)
+        self.fp8 = Fp8(self.ctx)

@@ -687,6 +687,109 @@ int dh_pages_table(const dh_pages* p, uint32_t seq, uint64_t* tokens, uint32_t* 
 uint32_t dh_pages_free(const dh_pages* p);
 uint32_t dh_pages_refs(const dh_pages* p, uint32_t page);
 
+/* ======================================================================
+ * 8-bit floating point: rows and weights as e4m3 codes with a power-of-two
+ * scale for each block of 128, and the matrix product of such codes. decide
+ * has no counterpart: its GEMM path is fp16 (kernels/gemm.rs:126-176). Codes
+ * take half of fp16's bytes and their products run at twice its rate.
+ *
+ * A matrix of K columns:
+ *   codes   [rows][ld] bytes, OCP e4m3 numbers; columns from K to the next
+ *           multiple of DH_FP8_BLOCK are zero
+ *   scales  [ceil(K / 512)][lds][4] bytes: byte b of entry [j][r] is e + 127
+ *           for the scale 2^e of columns 128 (4 j + b) .. + 127 of row r
+ *           (activations) or of rows 128 r .. + 127 (weights); 0 .. 254. Bytes
+ *           of blocks that lie wholly behind K are not read.
+ * The value of a code is code x scale. The functions that code values choose
+ * the smallest e >= -100 that brings the block's largest finite magnitude to
+ * at most 448; each code is then one rounding (to nearest, ties to even) of
+ * its value. A value that is not finite becomes the code 0x7f, NaN.
+ * ====================================================================== */
+#define DH_FP8_BLOCK 128u
+
+typedef struct dh_fp8_matrix {
+  void* codes;   /* device memory, 16-byte aligned */
+  void* scales;  /* device memory, 16-byte aligned */
+  uint32_t ld;   /* a multiple of 16 covering K in whole blocks, at most 2^23 */
+  uint32_t lds;  /* a multiple of 4 covering the rows (activations) or blocks of rows (weights) */
+} dh_fp8_matrix;
+
+/* Codes `rows` rows of k columns, x[r * ldx + c] with dtype 0 fp16, 1 bf16,
+ * 2 fp32, with a scale for each row and block of columns. With norm_w (fp32
+ * [k]) each row is first normed as dh_rmsnorm_rows does, x * (mean(x^2) +
+ * eps)^-1/2 * (add_one ? 1 + w : w), in 64 bits and rounded to fp32. Writes the
+ * codes of columns 0 .. k in whole blocks (zeros behind k) and the scale
+ * entries of the rows (127 for blocks behind k). Contract: ldx covers k and is
+ * a multiple of 8; x and norm_w 16-byte aligned; eps > 0 with norm_w. */
+int dh_fp8_quant_rows(dh_ctx* ctx, void* stream, const void* x, uint32_t ldx, uint32_t dtype, const float* norm_w,
+                      uint32_t add_one, float eps, const dh_fp8_matrix* out, uint32_t rows, uint32_t k);
+/* The same for a weight of n rows, with a scale for each 128 rows x 128 columns. */
+int dh_fp8_quant_blocks(dh_ctx* ctx, void* stream, const void* w, uint32_t ldw, uint32_t dtype, const dh_fp8_matrix* out,
+                        uint32_t n, uint32_t k);
+
+/* y = epi(X . W^T) of the values that codes and scales stand for: x of m rows
+ * with a scale for each row, w of n rows with a scale for each 128 rows, k
+ * columns each; products exact, sums fp32, epilogues and y as dh_gemm_nt's.
+ * Contract: any m, n and k (n % 32 == 0 for SwiGLU); ldy % 4 == 0; y 16-byte
+ * (fp32 outputs) or 8-byte (fp16 outputs) aligned; a code of NaN makes its row
+ * (of x) or column (of w's row) NaN. Where there are few tiles K is divided and
+ * the parts are summed through `stream`'s split-K workspace (dh_gemm_fp8_ws, or
+ * an eager call of the same size, grows it). A row's bits depend on the call's
+ * m, n and k and on its own codes and scales alone. */
+int dh_gemm_fp8(dh_ctx* ctx, void* stream, const dh_fp8_matrix* x, const dh_fp8_matrix* w, void* y, uint32_t ldy,
+                uint32_t m, uint32_t n, uint32_t k, uint32_t epi);
+/* Grows `stream`'s split-K workspace to what dh_gemm_fp8 needs for n, k and any
+ * m up to max_m (at most DH_PLAN_MAX_ROWS). */
+int dh_gemm_fp8_ws(dh_ctx* ctx, void* stream, uint32_t max_m, uint32_t n, uint32_t k);
+
+/* ======================================================================
+ * Causal attention over packed sequences: the rows of several requests one
+ * behind another, each attending to its own sequence's keys. decide's attention
+ * takes one request's 16 heads of 256 dims (dh_attention); here heads, sizes
+ * and types are arguments, keys and values are read from the projections' rows
+ * (or any other), and a sequence may bring one row or thousands.
+ * ====================================================================== */
+/* The sequences of a call; device arrays. Sequence s has the rows q0[s] ..
+ * q0[s + 1] - 1 of q, gate and y and the rows k0[s] .. k0[s + 1] - 1 of k and v.
+ * Neither decreases, and entries past q_rows (k_rows) count as q_rows (k_rows).
+ * Rows of q that belong to no sequence are not read, and their y is left as it
+ * was. */
+typedef struct dh_packed_batch {
+  const uint32_t* q0; /* [seqs + 1] */
+  const uint32_t* k0; /* [seqs + 1]; may be q0: whole prompts */
+  uint32_t seqs;
+  uint32_t q_rows;    /* rows that q, gate and y hold (the launch is sized by it) */
+  uint32_t k_rows;    /* rows that k and v hold */
+  uint32_t max_k;     /* keys of the longest sequence, for the launch's division of long ones; a hint */
+} dh_packed_batch;
+
+/* y[r, h] = softmax_t(scale * q[r, h] . k[t, g]) . v[t, g] (x sigmoid(gate[r, h])),
+ * kv head g = h / (heads / kv_heads). Row i (from 0) of a sequence of nq rows
+ * and nk keys sees its keys 0 .. nk - nq + i: a whole prompt where nk = nq, the
+ * last rows of a longer one, down to a single token, where nq < nk; where
+ * nq > nk the first nq - nk rows see nothing and are zero, whatever their q and
+ * gate hold. dtype, of q, k, v and y: 0 fp16, 1 bf16; gate (may be NULL) fp32.
+ * Head h of a row at column h * head_dim; strides ldq, ldk, ldv, ldg, ldy in
+ * elements. Scores and softmax fp32; a weight relative to its row's largest is
+ * rounded to dtype as the operand of its product with v. Keys and values that
+ * no row sees may hold anything; what a row sees is followed through softmax,
+ * infinities and NaN among it.
+ * Contract: head_dim 64, 128 or 256; heads % kv_heads == 0, at most 1,024 heads
+ * a kv head; scale finite; ldq, ldk, ldv % 8 == 0, ldy, ldg % 4 == 0, each
+ * covering its heads; q, k, v and gate 16-byte, y 8-byte aligned. Few rows over
+ * many keys are divided across workgroups and merged through the context's
+ * forward-kernel workspace (dh_attention_packed_ws; an eager call of the same
+ * sizes also grows it). The same call gives the same bits. */
+int dh_attention_packed(dh_ctx* ctx, void* stream, const dh_packed_batch* batch, const void* q, uint32_t ldq,
+                        const void* k, uint32_t ldk, const void* v, uint32_t ldv, uint32_t dtype, uint32_t heads,
+                        uint32_t kv_heads, uint32_t head_dim, float scale, const float* gate, uint32_t ldg, void* y,
+                        uint32_t ldy);
+/* Grows `stream`'s forward-kernel workspace to what dh_attention_packed needs
+ * for calls of up to q_rows rows in up to `seqs` sequences (before a capture on
+ * that stream, for instance). */
+int dh_attention_packed_ws(dh_ctx* ctx, void* stream, uint32_t q_rows, uint32_t seqs, uint32_t heads, uint32_t kv_heads,
+                           uint32_t head_dim);
+
 #ifdef __cplusplus
 }
 #endif
