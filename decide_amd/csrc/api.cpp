@@ -507,9 +507,9 @@ int dh_warm_up(dh_ctx* ctx, void* stream, uint32_t max_m) {
   void* scratch = nullptr;
   const size_t xb = 16 * 128 * 2, wb = 512 * 64 * 2, yb = 16 * 512 * 4;
   const size_t gemm_bytes = (xb + wb + yb + 127) / 128 * 128;
-  hipError_t e = hipMalloc(&scratch, gemm_bytes + kv8_warm_bytes() + fp8_warm_bytes() + 512);
+  hipError_t e = hipMalloc(&scratch, gemm_bytes + kv8_warm_bytes() + fp8_warm_bytes() + packed_warm_bytes());
   if (e != hipSuccess) return fail(DH_ENOMEM, "dh_warm_up: %s", hipGetErrorString(e));
-  e = hipMemsetAsync(scratch, 0, gemm_bytes + kv8_warm_bytes() + fp8_warm_bytes() + 512, s);
+  e = hipMemsetAsync(scratch, 0, gemm_bytes + kv8_warm_bytes() + fp8_warm_bytes() + packed_warm_bytes(), s);
   int rc = hip_status(e, "dh_warm_up memset");
   char* base = (char*)scratch;
   for (int v = 0; v < dh::variant_count() && rc == DH_OK; ++v) {

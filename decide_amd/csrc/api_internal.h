@@ -49,8 +49,8 @@ enum : int {
   kKidConv, kKidConvState, kKidDelta, kKidGNorm, kKidQRope, kKidKVRope, kKidAttn, kKidEmbed, kKidFillAny,
   kKidDeltaChunk, kKidStream, kKidAttnCombine, kKidConvDelta, kKidAddNorm, kKidDeltaBlock,
   kKidRope, kKidKv8Append, kKidKv8Attn, kKidKv8Combine, kKidKv8Copy,
-  kKidFp8Rows, kKidFp8Blocks, kKidFp8Reduce, kKidPacked, kKidPackedMerge, kKidFp8Gemm,  // (and its variants behind it)
-  kKidCount = kKidFp8Gemm + 4
+  kKidFp8Rows, kKidFp8Blocks, kKidFp8Reduce, kKidPacked, kKidPackedWide, kKidPackedMerge, kKidFp8Gemm,  // (and its variants behind it)
+  kKidCount = kKidFp8Gemm + 5
 };
 static_assert(kKidCount <= 64, "kernel ids must fit dh_ctx::used");
 
@@ -81,9 +81,10 @@ int attention_run(dh_ctx* ctx, void* stream, const uint16_t* q, const uint16_t* 
 size_t kv8_warm_bytes();
 int kv8_warm(dh_ctx* ctx, hipStream_t s, void* mem);
 
-// The same for the 8-bit codes and their product, and for attention over packed sequences (512 zeroed bytes).
+// The same for the 8-bit codes and their product, and for attention over packed sequences (packed_warm_bytes()).
 size_t fp8_warm_bytes();
 int fp8_warm(dh_ctx* ctx, hipStream_t s, void* mem);
+size_t packed_warm_bytes();
 int packed_warm(dh_ctx* ctx, hipStream_t s, void* mem);
 
 }  // namespace dh_api

@@ -1,5 +1,6 @@
 // C ABI of attention over packed sequences (include/decide_hip.h, "Causal attention over packed sequences").
 // Contract violations return DH_EINVAL with a message; nothing is launched after a failed check.
+#include <algorithm>
 #include <cmath>
 
 #include "api_internal.h"
@@ -71,29 +72,54 @@ int dh_attention_packed(dh_ctx* ctx, void* stream, const dh_packed_batch* batch,
   a.kv_heads = kv_heads, a.group = heads / kv_heads;
   a.group_inv = ((1u << 21) + a.group - 1) / a.group;
   a.scale = scale;
-  a.slots = (uint32_t)((uint64_t)batch->q_rows * a.group / 256 + batch->seqs);
-  mark(ctx, kKidPacked);
-  return hip_status(dh::launch_packed_wide(a, head_dim, dtype == 1, (hipStream_t)stream), op);
+  const dh::PackPlan plan = dh::packed_plan(batch->q_rows, batch->seqs, heads, kv_heads, head_dim, batch->max_k, ctx->cus);
+  a.slots = plan.slots, a.runs = plan.runs, a.min_run = plan.min_run;
+  if (plan.ws_bytes) {
+    rc = ensure_aux(ctx, (hipStream_t)stream, plan.ws_bytes, &a.ws);
+    if (rc != DH_OK) return rc;
+    mark(ctx, kKidPackedMerge);
+  }
+  mark(ctx, plan.wide ? kKidPackedWide : kKidPacked);
+  return hip_status(plan.wide ? dh::launch_packed_wide(a, head_dim, dtype == 1, (hipStream_t)stream)
+                              : dh::launch_packed_narrow(a, head_dim, dtype == 1, (hipStream_t)stream),
+                    op);
 }
 
 int dh_attention_packed_ws(dh_ctx* ctx, void* stream, uint32_t q_rows, uint32_t seqs, uint32_t heads, uint32_t kv_heads,
                            uint32_t head_dim) {
-  (void)stream;
   int rc = check_shape("attention_packed_ws", q_rows, seqs, heads, kv_heads, head_dim);
   if (rc != DH_OK) return rc;
   if (!ctx) return fail(DH_EINVAL, "attention_packed_ws: null context");
-  return ok();
+  if (q_rows == 0 || seqs == 0) return ok();
+  // Runs are as many whatever the call; there are at most kPackSlots tiles.
+  const uint64_t bytes =
+      dh::packed_run_bytes(std::max(1u, ctx->cus / kv_heads), dh::kPackSlots, kv_heads, head_dim);
+  float* ws = nullptr;
+  return ensure_aux(ctx, (hipStream_t)stream, bytes, &ws);
 }
 
 }  // extern "C"
 
 namespace dh_api {
 
+size_t packed_warm_bytes() { return dh::packed_run_bytes(1, 1, 1, 64) + 64; }
+
 int packed_warm(dh_ctx* ctx, hipStream_t s, void* mem) {
   // one row that belongs to no sequence: every kernel ends at once
-  const uint32_t* const zeros = (const uint32_t*)mem;
-  const dh_packed_batch batch{zeros, zeros, 1, 1, 1, 1};
-  return dh_attention_packed(ctx, s, &batch, mem, 64, mem, 64, mem, 64, 0, 1, 1, 64, 1.f, nullptr, 0, (char*)mem + 256, 64);
+  dh::PackArgs a{};
+  a.q = a.k = a.v = (const uint16_t*)mem;
+  a.q0 = a.k0 = (const uint32_t*)mem;
+  a.y = (uint16_t*)mem;
+  a.ws = (float*)mem;
+  a.ldq = a.ldk = a.ldv = a.ldy = 64;
+  a.seqs = a.q_rows = a.k_rows = a.kv_heads = a.group = a.slots = a.runs = a.min_run = 1;
+  a.group_inv = 1u << 21;
+  mark(ctx, kKidPackedWide);
+  mark(ctx, kKidPacked);
+  mark(ctx, kKidPackedMerge);
+  int rc = hip_status(dh::launch_packed_wide(a, 64, false, s), "attention_packed");
+  if (rc == DH_OK) rc = hip_status(dh::launch_packed_narrow(a, 64, false, s), "attention_packed");
+  return rc;
 }
 
 }  // namespace dh_api

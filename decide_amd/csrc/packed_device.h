@@ -61,6 +61,16 @@ __device__ __forceinline__ float scale_into(s8 (&q)[N], float scale) {
   return 1.0f;
 }
 
+// Chunk c of 16 bytes of K's row t lies at c ^ pack_k_key(t): both 8 lanes and 16 that read chunk c of as many rows read
+// different banks. Of V's row at c ^ pack_v_key(t): a transposing read takes 64 bytes of each of four rows.
+template <int D>
+__device__ __forceinline__ uint32_t pack_k_key(uint32_t t) {
+  return D == 64 ? (t & 7) ^ (t >> 3 & 1) : t & 15;
+}
+template <int D>
+__device__ __forceinline__ uint32_t pack_v_key(uint32_t t) {
+  return D == 64 ? (t >> 1 & 1) * 4 : (t & 3) * 4;
+}
 // Combined over the two halves of a wave: lanes r and r + 32 hold one pair's scores.
 __device__ __forceinline__ float max_of_halves(float x) {
   auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -99,16 +109,21 @@ struct PackTile {
 
 // Tile `slot` of a kv head: sequence s's tiles start at q0[s] * group / TILE + s, which leaves room for all before it.
 template <uint32_t TILE>
-__device__ __forceinline__ bool find_pack_tile(const PackArgs& a, uint32_t slot, PackTile& t) {
-  uint32_t begin, end;
-  const uint32_t s = kv_find_seq(a.q0, a.seqs, a.q_rows, slot, a.group, TILE, 1, begin, end);
-  if (s >= a.seqs || end <= begin) return false;
+__device__ __forceinline__ bool pack_tile_of(const PackArgs& a, uint32_t slot, uint32_t s, uint32_t begin, uint32_t end,
+                                             PackTile& t) {
+  if (end <= begin) return false;
   const uint32_t pairs = (end - begin) * a.group;
   const uint32_t first = (slot - (uint32_t)((uint64_t)begin * a.group / TILE) - s) * TILE;
   if (first >= pairs) return false;
   const uint32_t kb = min(a.k0[s], a.k_rows), ke = min(a.k0[s + 1], a.k_rows);
   t = PackTile{s, pairs - first, begin + first / a.group, first % a.group, begin, end, kb, ke > kb ? ke - kb : 0};
   return true;
+}
+template <uint32_t TILE>
+__device__ __forceinline__ bool find_pack_tile(const PackArgs& a, uint32_t slot, PackTile& t) {
+  uint32_t begin, end;
+  const uint32_t s = kv_find_seq(a.q0, a.seqs, a.q_rows, slot, a.group, TILE, 1, begin, end);
+  return s < a.seqs && pack_tile_of<TILE>(a, slot, s, begin, end, t);
 }
 // Row and head of the tile's pair k < 256. For x = extra + k < group + 256, x times the rounded 2^21 / group is off by less
 // than x, and x group < 2^21 for groups of at most 1,024: the quotient is exact. (The product stays below 2^32.)

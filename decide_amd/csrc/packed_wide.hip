@@ -2,31 +2,32 @@
 //
 //   y[r, h] = softmax_t(scale * q[r, h] . k[t, g]) . v[t, g] (x sigmoid(gate[r, h])),  t < keys - (rows behind r)
 //
-// Tiles of 32 WAVES (row, head) pairs of one kv head, 32 a wave; keys in blocks of 64, which all waves read from LDS.
+// Tiles of 128 (row, head) pairs of one kv head, 32 for each of four waves; keys in blocks of 32 T, which all waves read from LDS.
 //   * Everything is computed transposed, S^T = K Q^T and O^T = V^T P^T, on v_mfma_f32_32x32x16: lane (r, h), r = lane % 32, h
 //     = lane / 32, holds scores of ONE pair r, 16 of every 32 keys: 8 i + 4 h + j, i, j < 4. The largest and the sum of a
 //     pair are in its two lanes, and the weights are, as they are, the operand of P^T: eight a lane for 16 keys, 4 h + j and
 //     8 + 4 h + j. V's operand is to hold the same keys for each dim: two transposing reads of four rows of V each.
-//   * K and V go into LDS by DMA, a ring of NBUF blocks. 16-byte chunk c of K's row t lies at c ^ t % 8: eight lanes that
-//     read chunk c of eight rows read different banks. Of V's row at c ^ 4 (t % 4) (64 dims: 4 (t / 2 % 2)): a transposing
-//     read takes 64 bytes of each of four rows.
+//   * K and V go into LDS by DMA, two blocks in turn, their chunks swizzled (packed_device.h). Two workgroups share a CU, and so
+//     two waves a SIMD, which need not be in step: 8,192 rows of 32 heads over 8 of 128 dims 585 us; eight waves in one
+//     workgroup on a ring of four blocks 611, and with the two of a SIMD kept half a block apart 614; three workgroups with
+//     blocks of 32 keys 620.
 //   * The softmax's reference point moves only where a score exceeds it by 2^8, so O is rarely rescaled.
 //   * Keys past the sequence's end are its last one again, masked: another sequence's values are never touched.
 #include "packed_device.h"
 
 namespace dh {
 
-template <int D, bool BF16, int WAVES, int NBUF>
-__global__ __launch_bounds__(WAVES * 64) void packed_wide_kernel(PackArgs a) {
-  constexpr uint32_t kTile = 32 * WAVES, kBlock = 64;
-  constexpr uint32_t kRow = 2 * D, kBytes = kBlock * kRow;         // of a key, of a block's K (or V)
+template <int D, bool BF16>
+__global__ __launch_bounds__(256, 2) void packed_wide_kernel(PackArgs a) {
+  constexpr int T = D == 64 ? 4 : D == 128 ? 2 : 1;  // 64 KB of LDS: two workgroups a CU
+  constexpr uint32_t kTile = kPackWideTile, kWaves = kTile / 32, kBlock = 32 * T;
+  constexpr uint32_t kRow = 2 * D, kBytes = kBlock * kRow;      // of a key, of a block's K (or V)
   constexpr int KS = D / 16, DT = D / 32;
-  constexpr int kAhead = 3;             // LDS reads ahead of their products
-  constexpr int T = D == 256 ? 1 : 2;  // 32 T keys at a time (registers allow no more)
-  constexpr int kPieces = 2 * kBytes / 1024 / WAVES;               // DMAs of a wave for a block
-  constexpr uint32_t kChunks = D / 8, kRowsEach = 64 / kChunks;     // 16-byte chunks of a row, rows of a DMA
-  __shared__ __attribute__((aligned(1024))) char lds[NBUF * 2 * kBytes];
-  static_assert(NBUF * 2 * kBytes >= WAVES * 8192, "the outputs' exchange fits the ring");
+  constexpr int kAhead = D == 256 ? 3 : 3;                      // LDS reads ahead of their products
+  constexpr int kPieces = 2 * kBytes / 1024 / kWaves;           // DMAs of a wave for a block
+  constexpr uint32_t kChunks = D / 8, kRowsEach = 64 / kChunks;  // 16-byte chunks of a row, rows of a DMA
+  __shared__ __attribute__((aligned(1024))) char lds[2 * 2 * kBytes];
+  static_assert(2 * 2 * kBytes >= kWaves * 8192, "the outputs' exchange fits the ring");
   const uint32_t kvh = blockIdx.x % a.kv_heads, slot = a.slots - 1 - blockIdx.x / a.kv_heads;
   PackTile tile;
   if (!find_pack_tile<kTile>(a, slot, tile)) return;
@@ -49,29 +50,32 @@ __global__ __launch_bounds__(WAVES * 64) void packed_wide_kernel(PackArgs a) {
   }
   const float c = scale_into<BF16>(q, a.scale);
 
-  auto k_key = [](uint32_t t) { return t & 7; };
-  auto v_key = [](uint32_t t) { return D == 64 ? (t >> 1 & 1) * 4 : (t & 3) * 4; };
   const uint8_t* const kp = (const uint8_t*)(a.k + (size_t)tile.k_begin * a.ldk + kvh * D);
   const uint8_t* const vp = (const uint8_t*)(a.v + (size_t)tile.k_begin * a.ldv + kvh * D);
-  // What follows from the lane is formed where it is used: kept over the blocks it would spill, and a spill's reload waits for
-  // the DMAs.
-  auto lane_again = [] {
-    uint32_t x = threadIdx.x;
-    asm volatile("" : "+v"(x));
-    return x & 63;
-  };
+  // A DMA brings kRowsEach rows, a lane 16 bytes of one: piece p of a block's K (or V) its rows kRowsEach p on. A wave's pieces
+  // are 4 apart, which leaves a lane's chunk the same (but for K of 256 dims,
+  // where 8 rows on it is the other half's).
+  constexpr int kEach = kPieces / 2;  // of K and of V each
+  static_assert(kPieces % 2 == 0 && kEach * kWaves * kRowsEach == kBlock, "a wave's DMAs are K's, then V's");
+  const uint32_t t0 = wave * kRowsEach + lane / kChunks;
+  const uint32_t kchunk = (lane % kChunks ^ pack_k_key<D>(t0)) * 16, vchunk0 = (lane % kChunks ^ pack_v_key<D>(t0)) * 16;
+  const uint32_t klane = lane / kChunks * a.ldk * 2, vlane = lane / kChunks * a.ldv * 2;
   auto stage = [&](uint32_t b) {
-    const uint32_t lane = D == 256 ? lane_again() : threadIdx.x & 63;
-    const uint32_t to = lds0 + b % NBUF * 2 * kBytes, last = tile.keys - 1 - b * kBlock;
+    const uint32_t to = lds0 + b % 2 * 2 * kBytes, left = tile.keys - b * kBlock;
+    auto piece = [&](int i, const uint8_t* from, uint32_t ld, uint32_t row_at, uint32_t chunk) {
+      const uint32_t first = (kWaves * (i % kEach) + wave) * kRowsEach, at = to + (i / kEach) * kBytes + (kWaves * (i % kEach) + wave) * 1024;
+      const uint8_t* const base = from + (size_t)(b * kBlock) * ld * 2;
+      if (left >= kBlock) {
+        dma16(at, row_at + chunk, base + (size_t)first * ld * 2);
+      } else {  // keys past the end are the last one again
+        const uint32_t f = min(first, left - 1);
+        dma16(at, min(row_at, (left - 1 - f) * ld * 2) + chunk, base + (size_t)f * ld * 2);
+      }
+    };
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const uint32_t piece = i * WAVES + wave;
-      const bool of_k = piece < kBytes / 1024;
-      const uint32_t t = piece % (kBytes / 1024) * kRowsEach + lane / kChunks;
-      const uint32_t chunk = lane % kChunks ^ (of_k ? k_key(t) : v_key(t));
-      const uint32_t ld = of_k ? a.ldk : a.ldv;
-      dma16(to + piece * 1024, min(t, last) * ld * 2 + chunk * 16, (of_k ? kp : vp) + (size_t)b * kBlock * ld * 2);
-    }
+    for (int i = 0; i < kEach; ++i) piece(i, kp, a.ldk, klane, D == 256 ? kchunk ^ (i & 1) * 128 : kchunk);
+#pragma unroll
+    for (int i = kEach; i < kPieces; ++i) piece(i, vp, a.ldv, vlane, vchunk0);
   };
 
   f16v o[DT];
@@ -81,39 +85,40 @@ __global__ __launch_bounds__(WAVES * 64) void packed_wide_kernel(PackArgs a) {
     for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
   float m = -INFINITY, l = 0.f;
 
-#pragma unroll
-  for (uint32_t b = 0; b < NBUF - 1; ++b)
-    if (b < blocks) stage(b);
+  if (blocks) stage(0);
 #pragma unroll
   for (int x = 0; x < KS; ++x) asm volatile("" : "+v"(q[x]));  // no wait for Q in the loop: it would wait for the DMAs too
   for (uint32_t b = 0; b < blocks; ++b) {
-    if (b + NBUF - 2 < blocks)
-      wait_vm<(NBUF - 2) * kPieces>();
-    else
-      wait_vm<0>();
+    wait_vm<0>();
     __syncthreads();  // block b has landed, and everyone is done with block b - 1
-    if (b + NBUF - 1 < blocks) stage(b + NBUF - 1);
-    const char* const kb = lds + b % NBUF * 2 * kBytes;
-#pragma unroll 1
-    for (uint32_t k0 = b * kBlock; k0 < min(wmost, (b + 1) * kBlock); k0 += 32 * T) {
-      const char* const ks = kb + k0 % kBlock * kRow;
+    if (b + 1 < blocks) stage(b + 1);
+    const bool on = b * kBlock < wmost;  // some pair of the wave sees the block
+    const char* const ks = lds + b % 2 * 2 * kBytes;
+    s8 p[2 * T];
+    if (on) {
+      uint32_t sw = (h ^ pack_k_key<D>(r)) * 16;
+      if (D == 256) asm volatile("" : "+v"(sw));  // formed here: the hoisted addresses would spill
+      __builtin_amdgcn_s_setprio(1);
       f16v st[T];
 #pragma unroll
-      for (int t = 0; t < T; ++t) {
+      for (int t = 0; t < T; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) st[t][e] = 0.f;
-        auto read_k = [&](int x) { return *(const s8*)(ks + (32 * t + r) * kRow + x / 4 * 128 + (((2 * (x % 4) + h) ^ k_key(r)) * 16)); };
-        s8 k[kAhead + 1];
+      // Chunk 2 x + h of a key lies at byte 32 x ^ sw. Reads run kAhead products ahead; the barriers keep the compiler from
+      // moving them to their use.
+      auto read_k = [&](int i) { return *(const s8*)(ks + (32 * (i % T) + r) * kRow + ((32 * (i / T)) ^ sw)); };
+      s8 k[kAhead + 1];
 #pragma unroll
-        for (int x = 0; x < kAhead; ++x) k[x] = read_k(x);
+      for (int i = 0; i < kAhead; ++i) k[i] = read_k(i);
 #pragma unroll
-        for (int x = 0; x < KS; ++x) {
-          if (x + kAhead < KS) k[(x + kAhead) % (kAhead + 1)] = read_k(x + kAhead);
-          if (D == 256) __builtin_amdgcn_sched_barrier(0);
-          st[t] = mfma_16bit<BF16>(k[x % (kAhead + 1)], q[x], st[t]);
-        }
+      for (int i = 0; i < T * KS; ++i) {
+        if (i + kAhead < T * KS) k[(i + kAhead) % (kAhead + 1)] = read_k(i + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
+        st[i % T] = mfma_16bit<BF16>(k[i % (kAhead + 1)], q[i / T], st[i % T]);
       }
-      if (k0 + (32 * T - 1) >= wleast) {
+      __builtin_amdgcn_s_setprio(0);
+      const uint32_t k0 = b * kBlock;
+      if (k0 + (kBlock - 1) >= wleast) {
 #pragma unroll
         for (int t = 0; t < T; ++t)
 #pragma unroll
@@ -133,7 +138,6 @@ __global__ __launch_bounds__(WAVES * 64) void packed_wide_kernel(PackArgs a) {
         for (int i = 0; i < DT; ++i) o[i] *= alpha;
       }
       const float mref = m == -INFINITY ? 0.f : m;
-      s8 p[2 * T];
 #pragma unroll
       for (int x = 0; x < 2 * T; ++x) {
         float w[8];
@@ -144,27 +148,31 @@ __global__ __launch_bounds__(WAVES * 64) void packed_wide_kernel(PackArgs a) {
         }
         p[x] = pack8<BF16>(w);
       }
+    }
+    if (on) {
       // V: rows 16 x + 8 y + 4 h + i / 4 of lane i of 16, which gets four rows of dim 32 d + lane % 32
-      const uint32_t i16 = lane & 15, vrow = 4 * h + i16 / 4;
+      const uint32_t i16 = lane & 15, vrow = 4 * (lane >> 5) + i16 / 4;
       const char* const vb = ks + kBytes + vrow * kRow + (i16 & 1) * 8;
       const uint32_t vchunk = 2 * (lane >> 4 & 1) + (i16 >> 1 & 1);
       auto read_v = [&](int i) {
         typedef __attribute__((address_space(3))) s4* lds_s4;
         const int d = i / (2 * T);
-        const char* const vd = vb + d / 4 * 256 + ((4 * (d % 4) + vchunk) ^ v_key(vrow)) * 16 + 16 * (i % (2 * T)) * kRow;
+        const char* const vd = vb + d / 4 * 256 + ((4 * (d % 4) + vchunk) ^ pack_v_key<D>(vrow)) * 16 + 16 * (i % (2 * T)) * kRow;
         const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)vd);
         const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(vd + 8 * kRow));
         return s8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       };
+      __builtin_amdgcn_s_setprio(1);
       s8 v[kAhead + 1];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) v[i] = read_v(i);
 #pragma unroll
       for (int i = 0; i < 2 * T * DT; ++i) {
         if (i + kAhead < 2 * T * DT) v[(i + kAhead) % (kAhead + 1)] = read_v(i + kAhead);
-        if (D == 256) __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_sched_barrier(0);
         o[i / (2 * T)] = mfma_16bit<BF16>(v[i % (kAhead + 1)], p[i % (2 * T)], o[i / (2 * T)]);
       }
+      __builtin_amdgcn_s_setprio(0);
     }
   }
   __syncthreads();  // the outputs go where the blocks lay
@@ -201,8 +209,7 @@ __global__ __launch_bounds__(WAVES * 64) void packed_wide_kernel(PackArgs a) {
 namespace {
 template <int D, bool BF16>
 void wide_kernel(const PackArgs& a, hipStream_t s) {
-  constexpr int NBUF = D == 256 ? 2 : D == 128 ? 3 : 4;
-  hipLaunchKernelGGL((packed_wide_kernel<D, BF16, 8, NBUF>), dim3(a.kv_heads * a.slots), dim3(512), 0, s, a);
+  hipLaunchKernelGGL((packed_wide_kernel<D, BF16>), dim3(a.kv_heads * a.slots), dim3(256), 0, s, a);
 }
 }  // namespace
 

@@ -98,28 +98,34 @@ def attention(q, k, v, gate, scale, q0, k0, heads, kv_heads, half):
         a, b = min(q0[s], rows), min(q0[s + 1], rows)
         ka, kb = min(k0[s], len(k)), min(k0[s + 1], len(k))
         nq, nk = max(b - a, 0), max(kb - ka, 0)
-        for i in range(nq):
-            seen = max(0, nk - nq + i + 1)
-            for h in range(heads):
-                if seen == 0:
-                    y[a + i, h] = 0.0
-                    continue
-                kk, vv = k[ka:ka + seen, h // group], v[ka:ka + seen, h // group]
-                with np.errstate(invalid="ignore", over="ignore"):
-                    sc = scale * (kk @ q[a + i, h])
-                    p = np.exp(sc - sc.max())
-                    total = p.sum()
-                    y[a + i, h] = p @ vv / total
-                    # Scores: dim products and sums in fp32 (each addition off by at most 2 U of the terms' sum, whichever
-                    # way it rounds), the scale's two roundings and the difference from the reference point, up to 8 past
-                    # it, rounded once: 2 U |score| + 8 U. exp2's own error 2 U. The weight's rounding as an operand: half.
-                    ds = 2 * (dim + 4) * u * abs(scale) * (np.abs(kk) @ np.abs(q[a + i, h])) + 4 * u * np.abs(sc) + 16 * u
-                    # A score of -infinity weighs 0 exactly.
-                    ds = np.where(sc == -np.inf, 0.0, ds)
-                    # sums of `seen` weights and products, twice U each at most, in numerator and denominator; the division
-                    sums = (4 * seen + 8) * u
-                    err[a + i, h] = (p * (half + 2 * ds)) @ np.abs(vv) / total + \
-                        np.abs(y[a + i, h]) * (p @ (2 * ds) / total) + sums * (p @ np.abs(vv)) / total
+        seen = np.maximum(0, nk - nq + np.arange(nq) + 1)
+        hidden = np.arange(nk)[None] >= seen[:, None]
+        for h in range(heads if nq else 0):
+            kk, vv, qq = k[ka:kb, h // group], v[ka:kb, h // group], q[a:b, h]
+            none = seen == 0
+            with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
+                sc = np.where(hidden, -np.inf, scale * (qq @ kk.T))
+                top = np.where(none, 0.0, sc.max(1, initial=-np.inf))[:, None]
+                p = np.where(hidden, 0.0, np.exp(sc - top))
+                total = np.where(none, 1.0, p.sum(1))[:, None]
+                # a hidden value counts for nothing, whatever it is
+                bad = ~np.isfinite(vv)
+                val = p @ np.where(bad, 0.0, vv)
+                if bad.any():
+                    val = np.where(~hidden @ bad, np.nan, val)
+                size = p @ np.where(bad, 0.0, np.abs(vv)) / total
+                # Scores: dim products and sums in fp32 (each addition off by at most 2 U of the terms' sum, whichever way it
+                # rounds), the scale's two roundings and the difference from the reference point, up to 8 past it, rounded
+                # once: 2 U |score| + 8 U. exp2's own error 2 U. The weight's rounding as an operand: half.
+                ds = 2 * (dim + 4) * u * abs(scale) * (np.abs(qq) @ np.abs(kk).T) + 4 * u * np.abs(sc) + 16 * u
+                # A score of -infinity weighs 0 exactly.
+                pd = p * np.where(sc == -np.inf, 0.0, 2 * ds)
+                y[a:b, h] = np.where(none[:, None], 0.0, val / total)
+                # sums of `seen` weights and products, twice U each at most, in numerator and denominator; the division
+                sums = ((4 * seen + 8) * u)[:, None]
+                e = half * size + pd @ np.where(bad, 0.0, np.abs(vv)) / total + \
+                    np.abs(y[a:b, h]) * (pd.sum(1)[:, None] / total) + sums * size
+                err[a:b, h] = np.where(none[:, None], 0.0, e)
     if gate is not None:
         sees = np.zeros(rows, bool)
         for s in range(len(q0) - 1):

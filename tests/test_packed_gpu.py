@@ -129,6 +129,41 @@ def test_longer_sequences(gpu, kernels, stream, heads, kv, dim, dtype, nq, nk):
     Packed(nq, nk, heads, kv, dim, dtype).check(kernels, stream)
 
 
+WIDE = [  # enough (row, head) pairs for the tiles of many rows
+    (32, 2, 128, "bf16", [610], [610]), (48, 6, 256, "f16", [300, 1, 170], [300, 500, 200]), (64, 64, 64, "f16", [400], [400]),
+    (48, 2, 64, "bf16", [129, 0, 380], [700, 5, 380]), (24, 3, 128, "f16", [500, 65, 300], [500, 64, 1100]),
+    (40, 8, 256, "bf16", [33, 600], [40, 600]),
+]
+
+
+@pytest.mark.parametrize("heads,kv,dim,dtype,nq,nk", WIDE)
+def test_many_rows(gpu, kernels, stream, heads, kv, dim, dtype, nq, nk):
+    assert sum(nq) * heads // 32 >= (9 if dim == 128 else 11) * 256 // 4  # the planner takes wide tiles from here on
+    Packed(nq, nk, heads, kv, dim, dtype, gate=len(nq) > 1).check(kernels, stream)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_many_rows_of_odd_scales_and_contents(gpu, kernels, stream, dim):
+    """A negative scale and none; keys of -infinity and NaN; rows that see nothing; what is not finite in another sequence."""
+    for scale in (-0.4, 0.0):
+        Packed([90] * 3, [90] * 3, 96, 4, dim, "f16", scale=scale).check(kernels, stream)
+    p = Packed([400], [400], 64, 2, dim, "f16", gate=False)
+    p.qr[:], p.q[:] = np.abs(p.qr), np.abs(p.q)
+    for at, value in ((p.k0[0] + 5, -np.inf), (p.k0[0] + 398, np.nan), (p.k0[0], -np.inf)):
+        p.kr[at], p.k[at] = value, value
+    got = p.check(kernels, stream)
+    assert np.isnan(got[[0, -1, -2]]).all() and np.isfinite(got[1:-2]).all()
+    clean, bad = (Packed([200, 100, 100], [200, 20, 100], 64, 4, dim, "bf16") for _ in range(2))
+    bad.kr[bad.k0[1]:bad.k0[2]:7] = bad.vr[bad.k0[1]:bad.k0[2]:5] = 0x7f80
+    bad.qr[bad.q0[1]:bad.q0[1] + 9] = 0x7fc0
+    bad.g[bad.q0[1]:bad.q0[1] + 9] = np.nan
+    a, b = clean.run(kernels, stream), bad.run(kernels, stream)
+    for s in (0, 2):
+        rows = slice(int(clean.q0[s]), int(clean.q0[s + 1]))
+        assert np.array_equal(a[rows], b[rows]) and np.isfinite(a[rows]).all()
+    assert (b[bad.q0[1]:bad.q0[1] + 80] == 0).all() and (a[bad.q0[1]:bad.q0[1] + 80] == 0).all()
+
+
 @pytest.mark.parametrize("heads", [100, 257])
 def test_groups_wider_than_a_tile(gpu, kernels, stream, heads):
     Packed([1, 3], [70, 3], heads, 1, 64, "f16").check(kernels, stream)
@@ -232,8 +267,8 @@ def test_warm_up_loads_packed_attention(gpu, stream):
     k = Kernels()
     k.gemm.warm_up(stream, 64)
     loaded = k.gemm.fast_pipelines()
-    for nq, nk in (([1], [3000]), ([700], [700]), ([5], [5])):
-        Packed(nq, nk, 4, 2, 128, "f16").run(k, stream)
+    for nq, nk, heads in (([1], [3000], 4), ([700], [700], 32), ([5], [5], 4)):
+        Packed(nq, nk, heads, 2, 128, "f16").run(k, stream)
     assert k.gemm.fast_pipelines() == loaded
     k.ctx.close()
 
@@ -241,7 +276,7 @@ def test_warm_up_loads_packed_attention(gpu, stream):
 def test_the_same_call_gives_the_same_bits_on_any_stream(gpu):
     k = Kernels()
     ps = [Packed(nq, nk, 8, 2, 128, "bf16", seed=i) for i, (nq, nk) in
-          enumerate([([1, 1], [3000, 700]), ([1] * 5, [900] * 5), ([200, 70], [200, 70])])]
+          enumerate([([1, 1], [3000, 700]), ([1] * 5, [900] * 5), ([2000, 700], [2000, 700]), ([200, 70], [200, 70])])]
     wants = [p.run(k, 0) for p in ps]
     streams = [Stream() for _ in ps]
     ys = [p.blank() for p in ps]
