@@ -174,7 +174,9 @@ class Product:
         x, w = (np.abs(np.pad(ref.values(*a, self.k), ((0, 0), (0, up(self.k, 128) - self.k))))
                 for a in ((self.x, self.ex, 1), (self.w, self.ew, 128)))
         err = 2 * U * (self.k + 32) * (x @ w.T)
-        if f16:
+        if f16 and x.shape[0] * w.shape[0] > 1 << 21:  # at most the largest of each side's eight
+            err += 7 * 2.0 ** -13 * (x.reshape(len(x), -1, 8).max(2) @ w.reshape(len(w), -1, 8).max(2).T)
+        elif f16:
             for c in range(0, x.shape[1], 8):
                 err += 7 * 2.0 ** -13 * (x[:, None, c:c + 8] * w[None, :, c:c + 8]).max(2)
         return err
@@ -238,6 +240,20 @@ def test_product_with_fp16_outputs(gpu, kernels, stream, m, n, k):
         err = err.reshape(m, -1) + 16 * U * np.abs(ref.swiglu(want))
         sw = ref.swiglu(want)
         assert as_fp16(got, sw, err)
+
+
+def test_product_with_fp16_outputs_in_the_largest_tiles(gpu, kernels, stream):
+    m, n, k = 2053, 4128, 650
+    p = Product(m, n, k, spread=0.3)
+    want, bound = p.want(), p.bound(True)
+    assert as_fp16(p.run(kernels, stream, Epilogue.StoreF16), want, bound)
+    p = Product(m, 4099, k, codes=lambda rng, shape: rng.integers(-8, 9, shape).astype(np.float64))
+    with np.errstate(over="ignore"):
+        assert np.array_equal(p.run(kernels, stream, Epilogue.StoreF16), p.want().astype(np.float16).astype(np.float64))
+    p = Product(m, n, k, codes=lambda rng, shape: rng.integers(-2, 3, shape).astype(np.float64) / 64)
+    want = p.want()
+    sw = ref.swiglu(want)  # exact sums: silu's and the product's own roundings
+    assert as_fp16(p.run(kernels, stream, Epilogue.SwigluF16), sw, 16 * U * np.abs(sw))
 
 
 @pytest.mark.parametrize("m,n,k", [(5, 40, 300), (70, 130, 512), (200, 200, 2050), (1100, 96, 700), (1200, 257, 384)])
