@@ -23,6 +23,7 @@ int check_matrix(const char* op, const char* what, const dh_fp8_matrix* x, uint6
   if ((x->codes && !aligned(x->codes, 16)) || (x->scales && !aligned(x->scales, 16)))
     return fail(DH_EINVAL, "%s: codes and scales of %s must be 16-byte aligned", op, what);
   if (x->ld > 1u << 23) return fail(DH_EINVAL, "%s: row stride %u of %s exceeds 2^23", op, x->ld, what);
+  if (x->lds > 1u << 26) return fail(DH_EINVAL, "%s: scale stride %u of %s exceeds 2^26", op, x->lds, what);
   return DH_OK;
 }
 

@@ -99,6 +99,60 @@ __device__ __forceinline__ float weight_of_state(float m, float top) {
 }
 __device__ __forceinline__ float sigmoid_of(float x) { return 1.0f / (1.0f + __expf(-x)); }
 
+// Masked weights are zero, and zero times an infinity or NaN is NaN: where some pair does not see all keys of a block, their
+// values are looked through first (two VALU operations for two of them), and where one is not finite, infinities are added for the
+// pairs that see it and zero takes its place. Infinities are made as products of bfloat16's largest number and the same again,
+// which overflow; a NaN is an infinity of either sign.
+// Is any of the 16 N bytes of LDS a lane, from `at` on, 1,024 apart, not finite?
+template <bool BF16, int N>
+__device__ __forceinline__ bool any_not_finite(const char* at) {
+  typedef unsigned short u2s __attribute__((ext_vector_type(2)));
+  u2s most = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const s8 v = *(const s8*)(at + i * 1024);
+#pragma unroll
+    for (int e = 0; e < 8; e += 2)
+      most = __builtin_elementwise_max(most, u2s{(unsigned short)v[e], (unsigned short)v[e + 1]} & (unsigned short)0x7fff);
+    if (i % 4 == 3) asm volatile("" : "+v"(most) : : "memory");
+  }
+  return __any(max(most[0], most[1]) >= (BF16 ? 0x7f80 : 0x7c00));
+}
+// Zero in their place.
+template <bool BF16, int N>
+__device__ __forceinline__ void clear_not_finite(char* at) {
+#pragma unroll 1
+  for (int i = 0; i < N; ++i) {
+    s8 v = *(const s8*)(at + i * 1024);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (v[e] & 0x7fff) >= (BF16 ? 0x7f80 : 0x7c00) ? (short)0 : v[e];
+    *(s8*)(at + i * 1024) = v;
+  }
+}
+// The infinities; value(d, x) is V's operand, sees(x, e) whether the lane's pair sees key e of operand x.
+template <bool BF16, int X, int DT, class Value, class Sees>
+__device__ __forceinline__ void add_infinities(f16v (&o)[DT], Value value, Sees sees) {
+  constexpr short kInf = BF16 ? 0x7f80 : 0x7c00, kNegInf = (short)(kInf | 0x8000);
+  constexpr short kLargest = 0x7f7f, kNegLargest = (short)0xff7f;
+#pragma unroll
+  for (int d = 0; d < DT; ++d) {
+#pragma unroll
+    for (int x = 0; x < X; ++x) {
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        s8 v = value(d, x), w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e] = (v[e] & 0x7fff) >= kInf && v[e] != (part ? kInf : kNegInf) ? (part ? kNegLargest : kLargest) : (short)0;
+          w[e] = sees(x, e) ? kLargest : (short)0;
+        }
+        o[d] = mfma_16bit<true>(v, w, o[d]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+}
+
 // Pairs (row, head of the group) of one kv head, row by row, from the tile's first on.
 struct PackTile {
   uint32_t seq;

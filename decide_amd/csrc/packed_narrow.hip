@@ -232,17 +232,26 @@ __global__ __launch_bounds__(WAVES * 64, 1) void packed_narrow_kernel(PackArgs a
       const uint32_t i16 = lane & 15, vrow = 4 * h + i16 / 4;
       const char* const vb = ks + kBytes + vrow * kRow + (i16 & 1) * 8;
       const uint32_t vchunk = 2 * (lane >> 4 & 1) + (i16 >> 1 & 1);
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const char* const vd = vb + d / 4 * 256 + ((4 * (d % 4) + vchunk) ^ pack_v_key<D>(vrow)) * 16;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          typedef __attribute__((address_space(3))) s4* lds_s4;
-          const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(vd + 16 * x * kRow));
-          const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(vd + (16 * x + 8) * kRow));
-          o[d] = mfma_16bit<BF16>(s8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, p[x], o[d]);
+      auto read_v = [&](int d, int x) {
+        typedef __attribute__((address_space(3))) s4* lds_s4;
+        const char* const vd = vb + d / 4 * 256 + ((4 * (d % 4) + vchunk) ^ pack_v_key<D>(vrow)) * 16 + 16 * x * kRow;
+        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)vd);
+        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(vd + 8 * kRow));
+        return s8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      };
+      if (k0 + 31 >= least) {  // values that not all pairs see
+        char* const at = lds + ((wave * kRing + s % kRing) * 2 + 1) * kBytes + lane * 16;
+        if (any_not_finite<BF16, kPieces>(at)) {
+          const int ahead = (int)(seen - k0 - 4 * h);  // keys that the lane sees from its first on
+          add_infinities<BF16, 2>(o, read_v, [&](int x, int e) { return 16 * x + 8 * (e / 4) + e % 4 < ahead; });
+          clear_not_finite<BF16, kPieces>(at);
+          asm volatile("" ::: "memory");  // the wave's own keys: LDS keeps its order
         }
       }
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) o[d] = mfma_16bit<BF16>(read_v(d, x), p[x], o[d]);
       if (mine(s + kRing)) {
         wait_lgkm<0>();
         stage(s + kRing, true);
@@ -380,7 +389,7 @@ hipError_t launch_packed_narrow(const PackArgs& a, uint32_t head_dim, bool bf16,
 // heads over 8 of 128, 600 keys 10.9 us against 9.9, 4,096 keys 12 against 38; 16 over 4 of 256, 8 rows of up to 1,000 keys 24
 // against 21, one of 2,000 17 against 34; 200 rows behind 6,000 keys (100 tiles) 66 against 91; 32 over 8 of 128, 4 x 64 rows
 // behind 3,000 keys (256 tiles) 43 against 33. Single tokens make a tile a sequence, mostly empty: 64 of up to 4,096 keys
-// (64 full tiles' pairs) 61 against 65.
+// (64 full tiles' pairs) 61 against 65. More kv heads than half of the CUs would leave a head one run.
 PackPlan packed_plan(uint32_t q_rows, uint32_t seqs, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_k,
                      uint32_t cus) {
   PackPlan p;
@@ -389,7 +398,7 @@ PackPlan packed_plan(uint32_t q_rows, uint32_t seqs, uint32_t heads, uint32_t kv
   p.wide = full >= (head_dim == 128 ? 9ull : 11ull) * cus / 4;
   p.slots = (uint32_t)(pairs / (p.wide ? kPackWideTile : kPackTile) + seqs);
   const uint32_t least = head_dim == 256 ? 1024 : head_dim == 128 ? 768 : 1536;
-  if (p.wide || p.slots > kPackSlots || max_k < least || full >= cus / 2) return p;
+  if (p.wide || p.slots > kPackSlots || max_k < least || full >= cus / 2 || kv_heads > cus / 2) return p;
   p.runs = std::max(1u, cus / kv_heads);
   p.min_run = 2;
   p.ws_bytes = packed_run_bytes(p.runs, p.slots, kv_heads, head_dim);

@@ -8,10 +8,13 @@
 //     pair are in its two lanes, and the weights are, as they are, the operand of P^T: eight a lane for 16 keys, 4 h + j and
 //     8 + 4 h + j. V's operand is to hold the same keys for each dim: two transposing reads of four rows of V each.
 //   * K and V go into LDS by DMA, two blocks in turn, their chunks swizzled (packed_device.h). Two workgroups share a CU, and so
-//     two waves a SIMD, which need not be in step: 8,192 rows of 32 heads over 8 of 128 dims 585 us; eight waves in one
-//     workgroup on a ring of four blocks 611, and with the two of a SIMD kept half a block apart 614; three workgroups with
-//     blocks of 32 keys 620.
+//     two waves a SIMD, which need not be in step: 8,192 rows of 32 heads over 8 of 128 dims 517 us (1,060 TF); when it took
+//     585, eight waves in one workgroup on a ring of four blocks took 611, and with the two of a SIMD kept half a block apart
+//     614; three workgroups with blocks of 32 keys 620. Matrix and vector instructions (the softmax) bound it, 45 and 42 %
+//     of the cycles, and they hardly overlap.
 //   * The softmax's reference point moves only where a score exceeds it by 2^8, so O is rarely rescaled.
+//   * Of 256 dims, 24 prompts of up to 2,307 rows and 16 heads over 4, 19.5 k rows in all, with gates: 400 us; there the bytes of
+//     Q, y and the gates alone are 161 us.
 //   * Keys past the sequence's end are its last one again, masked: another sequence's values are never touched.
 #include "packed_device.h"
 
@@ -23,10 +26,11 @@ __global__ __launch_bounds__(256, 2) void packed_wide_kernel(PackArgs a) {
   constexpr uint32_t kTile = kPackWideTile, kWaves = kTile / 32, kBlock = 32 * T;
   constexpr uint32_t kRow = 2 * D, kBytes = kBlock * kRow;      // of a key, of a block's K (or V)
   constexpr int KS = D / 16, DT = D / 32;
-  constexpr int kAhead = D == 256 ? 3 : 3;                      // LDS reads ahead of their products
+  constexpr int kAhead = D == 256 ? 2 : 3;  // LDS reads ahead of their products: as many as registers are left for
   constexpr int kPieces = 2 * kBytes / 1024 / kWaves;           // DMAs of a wave for a block
   constexpr uint32_t kChunks = D / 8, kRowsEach = 64 / kChunks;  // 16-byte chunks of a row, rows of a DMA
   __shared__ __attribute__((aligned(1024))) char lds[2 * 2 * kBytes];
+  __shared__ uint32_t odd[kWaves];
   static_assert(2 * 2 * kBytes >= kWaves * 8192, "the outputs' exchange fits the ring");
   const uint32_t kvh = blockIdx.x % a.kv_heads, slot = a.slots - 1 - blockIdx.x / a.kv_heads;
   PackTile tile;
@@ -34,11 +38,12 @@ __global__ __launch_bounds__(256, 2) void packed_wide_kernel(PackArgs a) {
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t r = lane & 31, h = lane >> 5;
+  auto same = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
   uint32_t row, head;
   pack_pair(a, tile, kvh, min(kTile, tile.pairs) - 1, row, head);
   const uint32_t most = pack_seen(tile, row), blocks = (most + kBlock - 1) / kBlock;
   pack_pair(a, tile, kvh, min(32 * wave + r, tile.pairs - 1), row, head);
-  const uint32_t seen = pack_seen(tile, row);
+  const uint32_t seen = pack_seen(tile, row), least = same(pack_seen(tile, tile.row));
   const uint32_t wmost = 32 * wave < tile.pairs ? max_of_wave(seen) : 0, wleast = ~max_of_wave(~seen);
 
   // Q: dims 16 x + 8 h .. + 7 of pair r
@@ -149,26 +154,49 @@ __global__ __launch_bounds__(256, 2) void packed_wide_kernel(PackArgs a) {
         p[x] = pack8<BF16>(w);
       }
     }
+    // V: rows 16 x + 8 y + 4 h + i / 4 of lane i of 16, which gets four rows of dim 32 d + lane % 32
+    auto read_v = [&](int i, uint32_t lane) {
+      typedef __attribute__((address_space(3))) s4* lds_s4;
+      const uint32_t i16 = lane & 15, vrow = 4 * (lane >> 5) + i16 / 4, vchunk = 2 * (lane >> 4 & 1) + (i16 >> 1 & 1);
+      const int d = i / (2 * T);
+      const char* const vd = ks + kBytes + vrow * kRow + (i16 & 1) * 8 + d / 4 * 256 +
+                             ((4 * (d % 4) + vchunk) ^ pack_v_key<D>(vrow)) * 16 + 16 * (i % (2 * T)) * kRow;
+      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)vd);
+      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(vd + 8 * kRow));
+      return s8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
+    if (b * kBlock + (kBlock - 1) >= least) {  // values that not all pairs of the tile see: a quarter of them for each wave
+      uint32_t here = lane;
+      if (D == 256) asm volatile("" : "+v"(here));  // formed here: hoisted addresses and masks would spill
+      char* const mine = lds + b % 2 * 2 * kBytes + kBytes + wave * (kBytes / kWaves) + here * 16;
+      const bool found = any_not_finite<BF16, kBytes / kWaves / 1024>(mine);
+      if (lane == 0) odd[wave] = found;
+      wait_lgkm<0>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (same(odd[0] | odd[1] | odd[2] | odd[3])) {
+        if (on) {
+          int ahead = (int)(seen - b * kBlock - 4 * (here >> 5));  // keys that the lane sees from its first on
+          add_infinities<BF16, 2 * T>(o,
+                                      [&](int d, int x) {
+                                        if (D == 256) asm volatile("" : "+v"(ahead));
+                                        return read_v(2 * T * d + x, here);
+                                      },
+                                      [&](int x, int e) { return 16 * x + 8 * (e / 4) + e % 4 < ahead; });
+        }
+        __syncthreads();
+        clear_not_finite<BF16, kBytes / kWaves / 1024>(mine);
+        __syncthreads();
+      }
+    }
     if (on) {
-      // V: rows 16 x + 8 y + 4 h + i / 4 of lane i of 16, which gets four rows of dim 32 d + lane % 32
-      const uint32_t i16 = lane & 15, vrow = 4 * (lane >> 5) + i16 / 4;
-      const char* const vb = ks + kBytes + vrow * kRow + (i16 & 1) * 8;
-      const uint32_t vchunk = 2 * (lane >> 4 & 1) + (i16 >> 1 & 1);
-      auto read_v = [&](int i) {
-        typedef __attribute__((address_space(3))) s4* lds_s4;
-        const int d = i / (2 * T);
-        const char* const vd = vb + d / 4 * 256 + ((4 * (d % 4) + vchunk) ^ pack_v_key<D>(vrow)) * 16 + 16 * (i % (2 * T)) * kRow;
-        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)vd);
-        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(vd + 8 * kRow));
-        return s8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      };
       __builtin_amdgcn_s_setprio(1);
       s8 v[kAhead + 1];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) v[i] = read_v(i);
+      for (int i = 0; i < kAhead; ++i) v[i] = read_v(i, lane);
 #pragma unroll
       for (int i = 0; i < 2 * T * DT; ++i) {
-        if (i + kAhead < 2 * T * DT) v[(i + kAhead) % (kAhead + 1)] = read_v(i + kAhead);
+        if (i + kAhead < 2 * T * DT) v[(i + kAhead) % (kAhead + 1)] = read_v(i + kAhead, lane);
         __builtin_amdgcn_sched_barrier(0);
         o[i / (2 * T)] = mfma_16bit<BF16>(v[i % (kAhead + 1)], p[i % (2 * T)], o[i / (2 * T)]);
       }

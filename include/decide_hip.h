@@ -698,8 +698,8 @@ uint32_t dh_pages_refs(const dh_pages* p, uint32_t page);
  *           multiple of DH_FP8_BLOCK are zero
  *   scales  [ceil(K / 512)][lds][4] bytes: byte b of entry [j][r] is e + 127
  *           for the scale 2^e of columns 128 (4 j + b) .. + 127 of row r
- *           (activations) or of rows 128 r .. + 127 (weights); 0 .. 254. Bytes
- *           of blocks that lie wholly behind K are not read.
+ *           (activations) or of rows 128 r .. + 127 (weights); 1 .. 254. Bytes
+ *           of blocks that lie wholly behind K count for nothing.
  * The value of a code is code x scale. The functions that code values choose
  * the smallest e >= -100 that brings the block's largest finite magnitude to
  * at most 448; each code is then one rounding (to nearest, ties to even) of
@@ -711,7 +711,7 @@ typedef struct dh_fp8_matrix {
   void* codes;   /* device memory, 16-byte aligned */
   void* scales;  /* device memory, 16-byte aligned */
   uint32_t ld;   /* a multiple of 16 covering K in whole blocks, at most 2^23 */
-  uint32_t lds;  /* a multiple of 4 covering the rows (activations) or blocks of rows (weights) */
+  uint32_t lds;  /* a multiple of 4 covering the rows (activations) or blocks of rows (weights), at most 2^26 */
 } dh_fp8_matrix;
 
 /* Codes `rows` rows of k columns, x[r * ldx + c] with dtype 0 fp16, 1 bf16,
@@ -729,7 +729,11 @@ int dh_fp8_quant_blocks(dh_ctx* ctx, void* stream, const void* w, uint32_t ldw, 
 
 /* y = epi(X . W^T) of the values that codes and scales stand for: x of m rows
  * with a scale for each row, w of n rows with a scale for each 128 rows, k
- * columns each; products exact, sums fp32, epilogues and y as dh_gemm_nt's.
+ * columns each; epilogues and y as dh_gemm_nt's. Products are exact and sums
+ * fp32; with fp16 outputs (SwiGLU among them) the products of each eight
+ * neighbouring columns are first added by the matrix instruction, which cuts
+ * what lies more than 13 bits below the largest of them (2^-13 of the largest
+ * product a term at most, a thirtieth of an fp16 rounding on ordinary data).
  * Contract: any m, n and k (n % 32 == 0 for SwiGLU); ldy % 4 == 0; y 16-byte
  * (fp32 outputs) or 8-byte (fp16 outputs) aligned; a code of NaN makes its row
  * (of x) or column (of w's row) NaN. Where there are few tiles K is divided and
@@ -771,9 +775,9 @@ typedef struct dh_packed_batch {
  * gate hold. dtype, of q, k, v and y: 0 fp16, 1 bf16; gate (may be NULL) fp32.
  * Head h of a row at column h * head_dim; strides ldq, ldk, ldv, ldg, ldy in
  * elements. Scores and softmax fp32; a weight relative to its row's largest is
- * rounded to dtype as the operand of its product with v. Keys and values that
- * no row sees may hold anything; what a row sees is followed through softmax,
- * infinities and NaN among it.
+ * rounded to dtype as the operand of its product with v. A row does not depend
+ * on keys and values that it does not see, whatever they hold; what it sees is
+ * followed through softmax, infinities and NaN among it.
  * Contract: head_dim 64, 128 or 256; heads % kv_heads == 0, at most 1,024 heads
  * a kv head; scale finite; ldq, ldk, ldv % 8 == 0, ldy, ldg % 4 == 0, each
  * covering its heads; q, k, v and gate 16-byte, y 8-byte aligned. Few rows over

@@ -268,6 +268,17 @@ def test_small_whole_numbers_are_exact(gpu, kernels, stream, m, n, k, epi):
         assert np.array_equal(got, want.astype(np.float32 if epi == Epilogue.StoreF32 else np.float16).astype(np.float64))
 
 
+@pytest.mark.parametrize("m,n", [(1300, 2600), (2050, 4100)])
+@pytest.mark.parametrize("epi", [Epilogue.StoreF32, Epilogue.StoreF16])
+def test_more_columns_than_their_scales_have_room_for(gpu, kernels, stream, m, n, epi):
+    """Small whole numbers again, exact, over 6,700 columns that few or no workgroups share; scales that all differ."""
+    k = 6700
+    p = Product(m, n, k, codes=lambda rng, shape: rng.integers(-4, 5, shape).astype(np.float64))
+    got, want = p.run(kernels, stream, epi), p.want()
+    with np.errstate(over="ignore"):
+        assert np.array_equal(got, want if epi == Epilogue.StoreF32 else want.astype(np.float16).astype(np.float64))
+
+
 @pytest.mark.parametrize("m,n,k", [(9, 64, 1100), (150, 140, 300), (1100, 300, 200)])
 @pytest.mark.parametrize("epi", [Epilogue.StoreF32, Epilogue.StoreF16])
 def test_nan_codes_reach_their_row_and_column_alone(gpu, kernels, stream, m, n, k, epi):

@@ -215,6 +215,39 @@ def test_keys_of_infinite_score_are_followed(gpu, kernels, stream, dim, nq, nk):
     assert np.isnan(got[0]).all() == (nq[0] == nk[0])
 
 
+HIDDEN = [  # narrow tiles, runs, rows that see nothing, wide tiles
+    (4, 2, [100], [100]), (4, 1, [37, 5], [90, 300]), (4, 2, [3], [2000]), (4, 2, [40], [11]), (64, 2, [400], [400]),
+    (64, 2, [150, 250], [60, 700]),
+]
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, "bf16"), (128, "f16"), (256, "bf16")])
+@pytest.mark.parametrize("heads,kv,nq,nk", HIDDEN)
+def test_values_that_a_row_does_not_see_may_be_anything(gpu, kernels, stream, dim, dtype, heads, kv, nq, nk):
+    """The last keys of each sequence have values of NaN and infinity in some columns: the rows before them, and other columns,
+    are as they would be without, to the bit; what sees an infinity is one, what sees a NaN or both infinities is NaN."""
+    clean, bad = (Packed(nq, nk, heads, kv, dim, dtype, size=0.1) for _ in range(2))
+    want = clean.run(kernels, stream)
+    marks = np.zeros((3, bad.keys, kv, dim), bool)  # +infinity, -infinity, NaN
+    for s in range(len(nq)):
+        k1 = bad.k0[s + 1]
+        for back, col, what in ((1, 5, 0), (2, dim - 1, 2), (9, 3, 1), (4, 3, 0), (7, 9, 1), (nk[s] // 8, 40, 2)):
+            marks[what, max(k1 - back - 1, bad.k0[s]), :, col] = True
+    for what, value in enumerate((np.inf, -np.inf, np.nan)):
+        bad.vr[marks[what]] = to_type(np.full(1, value), dtype)[0][0]
+    got = bad.run(kernels, stream)
+    seen = np.zeros((3, bad.rows, heads, dim), bool)
+    for s in range(len(nq)):
+        for i in range(nq[s]):
+            n = max(nk[s] - nq[s] + i + 1, 0)
+            seen[:, bad.q0[s] + i] = np.repeat(marks[:, bad.k0[s]:bad.k0[s] + n].any(1), heads // kv, 1)
+    plus, minus, nan = seen.reshape(3, bad.rows, -1)
+    rows = slice(bad.q0[0], bad.q0[-1])
+    nan = nan | plus & minus
+    want = np.where(nan, np.nan, np.where(plus, np.inf, np.where(minus, -np.inf, want)))
+    assert np.array_equal(got[rows], want[rows], equal_nan=True)
+
+
 def test_rows_that_see_nothing_are_zero_whatever_they_hold(gpu, kernels, stream):
     for dim in (64, 128, 256):
         p = Packed([9, 300], [4, 0], 4, 2, dim, "bf16")
@@ -223,6 +256,18 @@ def test_rows_that_see_nothing_are_zero_whatever_they_hold(gpu, kernels, stream)
         got = p.run(kernels, stream)
         assert (got[p.q0[0]:p.q0[0] + 5] == 0).all() and (got[p.q0[1]:p.q0[2]] == 0).all()
         assert np.isfinite(got[p.q0[0] + 5:p.q0[1]]).all()
+
+
+def test_as_many_heads_and_sequences_as_a_launch_takes(gpu, kernels, stream):
+    nq = [0] * 2040 + [1, 2, 0]
+    Packed(nq, [0] * 2040 + [3, 2, 1], 1024, 1024, 64, "f16", gate=False).check(kernels, stream)
+    p = Packed(nq, [0] * 2040 + [3, 2, 1], 1024, 1024, 64, "bf16", gate=False)
+    want = p.run(kernels, stream)
+    p.batch.c.max_k = 5000  # the hint that would have long sequences divided
+    y = p.blank()
+    p.call(kernels, stream, y)
+    sync()
+    assert np.array_equal(p.taken(to_host(y)), want, equal_nan=True)
 
 
 def test_k0_may_be_q0_and_entries_past_the_rows_end_there(gpu, kernels, stream):

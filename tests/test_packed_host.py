@@ -97,6 +97,14 @@ def test_packed_attention_refuses(kw, msg):
     _refused(_attn(**kw), msg)
 
 
+def test_scale_strides_past_their_addressing_are_refused():
+    wide = dict(lds=(1 << 26) + 4)
+    _refused(_rows(out=wide), "exceeds 2^26")
+    _refused(_blocks(out=wide), "exceeds 2^26")
+    _refused(_gemm(x=wide), "of x exceeds 2^26")
+    _refused(_gemm(w=wide), "of w exceeds 2^26")
+
+
 def test_sizing_calls_refuse():
     lib = _lib.load()
     _refused(lib.dh_gemm_fp8_ws(None, None, 16, 64, 64), "null context")
