@@ -80,7 +80,7 @@ int dh_fp8_quant_blocks(dh_ctx* ctx, void* stream, const void* w, uint32_t ldw, 
   int rc = check_source("fp8_quant_blocks", w, ldw, dtype, k);
   if (rc == DH_OK) rc = check_matrix("fp8_quant_blocks", "out", out, blocks, k);
   if (rc != DH_OK) return rc;
-  if (blocks * (((uint64_t)k + dh::kFp8Word - 1) / dh::kFp8Word) > kMaxThreads / 512)
+  if (blocks * (((uint64_t)k + dh::kFp8Word - 1) / dh::kFp8Word) > kMaxThreads / 1024)
     return fail(DH_EINVAL, "fp8_quant_blocks: %u rows of %u columns exceed one launch; split the call", n, k);
   if (!ctx) return fail(DH_EINVAL, "fp8_quant_blocks: null context");
   if (n == 0 || k == 0) return ok();

@@ -10,7 +10,7 @@
 // their four scales. Rows are coded from registers: each value is read once and its code written once, 8 bytes a lane.
 // With the norm a workgroup takes a row, whose sum of squares and whose normed values are formed in 64 bits: a value is
 // then one rounding to fp32 from exact, and which side of a scale's border it falls on does not depend on the order of a
-// sum. Bound by memory.
+// sum. Bound by memory: 16,383 x 9,216 fp16 values 78 us, 5.8 TB/s; eight normed rows of 2,560 4.2 us, a launch's time.
 #include <algorithm>
 
 #include "fp8.h"
@@ -60,6 +60,11 @@ struct Eight {
 #pragma unroll
       for (int i = 0; i < kWords; ++i) v[i / 4][i % 4] = part[i];
     }
+  }
+  // Values that are wanted again are formed again: as floats they would take twice the registers.
+  __device__ __forceinline__ void keep() {
+#pragma unroll
+    for (int i = 0; i < kWords / 4; ++i) asm volatile("" : "+v"(v[i]));
   }
   __device__ __forceinline__ float operator[](int i) const {
     if constexpr (kWords == 8) {
@@ -215,33 +220,37 @@ __global__ __launch_bounds__(256) void fp8_norm_rows_kernel(QuantArgs a) {
   }
 }
 
-// 128 rows and 512 columns a workgroup: eight waves of 16 rows, which stay in registers while the waves' largest values meet.
+// 128 rows and 512 columns a workgroup: 16 waves of eight rows, which stay in registers as they were read while the waves' largest
+// values meet. 18,432 x 2,560 from bf16: 29.9 us, 4.7 TB/s, as a large copy's; eight waves of 16 rows 31.2, and 37.3 with the
+// values kept as floats, whose registers leave a CU one workgroup.
 template <typename T>
-__global__ __launch_bounds__(512) void fp8_blocks_kernel(QuantArgs a) {
-  __shared__ uint32_t tops[8][4];
+__global__ __launch_bounds__(1024) void fp8_blocks_kernel(QuantArgs a) {
+  constexpr uint32_t kWaves = 16, kRows = kFp8Block / kWaves;
+  __shared__ uint32_t tops[kWaves][4];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, words = (a.k + kFp8Word - 1) / kFp8Word;
-  const uint32_t word = blockIdx.x % words, block = blockIdx.x / words, row0 = block * kFp8Block + wave * 16;
+  const uint32_t word = blockIdx.x % words, block = blockIdx.x / words, row0 = block * kFp8Block + wave * kRows;
   const uint32_t col = word * kFp8Word + 8 * lane, have = col < a.k ? a.k - col : 0;
   const uint32_t blocks = (a.k - word * kFp8Word + kFp8Block - 1) / kFp8Block;
-  Eight<T> e[16];
+  Eight<T> e[kRows];
 #pragma unroll
-  for (uint32_t r = 0; r < 16; ++r) e[r].load(a.x, (size_t)(row0 + r) * a.ldx + col, row0 + r < a.rows ? have : 0);
+  for (uint32_t r = 0; r < kRows; ++r) e[r].load(a.x, (size_t)(row0 + r) * a.ldx + col, row0 + r < a.rows ? have : 0);
   uint32_t top = 0;
 #pragma unroll
-  for (uint32_t r = 0; r < 16; ++r) {
+  for (uint32_t r = 0; r < kRows; ++r) {
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = e[r][i];
     top = max(top, top_of(v));
+    e[r].keep();
   }
   top = max16(top);
   if (lane % 16 == 0) tops[wave][lane / 16] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 8; ++w) top = max(top, tops[w][lane / 16]);
+  for (uint32_t w = 0; w < kWaves; ++w) top = max(top, tops[w][lane / 16]);
   const uint32_t b = scale_byte(top);
 #pragma unroll
-  for (uint32_t r = 0; r < 16; ++r) {
+  for (uint32_t r = 0; r < kRows; ++r) {
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = e[r][i];
@@ -284,11 +293,11 @@ hipError_t launch_fp8_quant_blocks(const void* w, uint32_t ldw, uint32_t dtype, 
   const QuantArgs a{w, nullptr, out.codes, out.scales, ldw, out.ld, out.lds, n, k, 0, 0.f};
   const dim3 grid((n + kFp8Block - 1) / kFp8Block * ((k + kFp8Word - 1) / kFp8Word));
   if (dtype == 0)
-    hipLaunchKernelGGL((fp8_blocks_kernel<Half>), grid, dim3(512), 0, s, a);
+    hipLaunchKernelGGL((fp8_blocks_kernel<Half>), grid, dim3(1024), 0, s, a);
   else if (dtype == 1)
-    hipLaunchKernelGGL((fp8_blocks_kernel<Bf16>), grid, dim3(512), 0, s, a);
+    hipLaunchKernelGGL((fp8_blocks_kernel<Bf16>), grid, dim3(1024), 0, s, a);
   else
-    hipLaunchKernelGGL((fp8_blocks_kernel<float>), grid, dim3(512), 0, s, a);
+    hipLaunchKernelGGL((fp8_blocks_kernel<float>), grid, dim3(1024), 0, s, a);
   return hipGetLastError();
 }
 
