@@ -27,8 +27,8 @@ constexpr uint32_t kPackTile = 32;       // (row, head) pairs of a tile of the k
 constexpr uint32_t kPackWideTile = 128;  // the same for many
 constexpr uint32_t kPackSlots = 2048;    // tiles that runs are dealt over (their steps lie in LDS)
 constexpr uint32_t kPackStep = 128;      // keys of a step
-// Steps of 32 keys that a wave of the kernel for few rows holds in LDS.
-constexpr int packed_ring(int head_dim, int waves) { return 131072 / (waves * 32 * head_dim * 2 * 2) > 3 ? 3 : 131072 / (waves * 32 * head_dim * 2 * 2); }
+// Steps of 32 keys that a wave of the kernel for few rows holds in LDS: 32 KB at most.
+constexpr int packed_ring(int head_dim) { return head_dim == 64 ? 3 : 256 / head_dim; }
 
 // How a call is computed: wide tiles, or narrow ones, a workgroup each or dealt in runs with their states in the workspace.
 struct PackPlan {

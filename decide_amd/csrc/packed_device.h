@@ -193,15 +193,21 @@ __device__ __forceinline__ uint32_t pack_seen(const PackTile& t, uint32_t row) {
   return t.keys > behind ? t.keys - behind : 0;
 }
 
-// eight dims of a pair's output, already over its sum
-template <bool BF16>
-__device__ __forceinline__ void store_pack8(const PackArgs& a, uint32_t row, uint32_t col, f4 v0, f4 v1, bool sees) {
-  if (a.gate) {
+// Eight dims of a pair's output, already over its sum, and of its gates, which are read long before they are wanted.
+struct Gate8 {
+  f4 g0, g1;
+  __device__ __forceinline__ void load(const PackArgs& a, uint32_t row, uint32_t col) {
     const f4* const g = (const f4*)(a.gate + (size_t)row * a.ldg + col);
-    const f4 g0 = g[0], g1 = g[1];
+    g0 = g[0], g1 = g[1];
+  }
+};
+template <bool BF16>
+__device__ __forceinline__ void store_pack8(const PackArgs& a, uint32_t row, uint32_t col, f4 v0, f4 v1, const Gate8& g,
+                                            bool sees) {
+  if (a.gate) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (sees) v0[e] *= sigmoid_of(g0[e]), v1[e] *= sigmoid_of(g1[e]);
+      if (sees) v0[e] *= sigmoid_of(g.g0[e]), v1[e] *= sigmoid_of(g.g1[e]);
     }
   }
   const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};

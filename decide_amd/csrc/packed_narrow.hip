@@ -39,7 +39,7 @@ template <int D, bool BF16, int WAVES, bool RUNS>
 __global__ __launch_bounds__(WAVES * 64, 1) void packed_narrow_kernel(PackArgs a) {
   constexpr uint32_t kRow = 2 * D, kBytes = 32 * kRow;  // of a key, of K (or V) of 32 keys
   constexpr int KS = D / 16, DT = D / 32;
-  constexpr int kRing = packed_ring(D, WAVES);
+  constexpr int kRing = packed_ring(D);
   constexpr int kPieces = kBytes / 1024;
   constexpr uint32_t kChunks = D / 8, kRowsEach = 64 / kChunks, kStep = 32 * WAVES;
   __shared__ __attribute__((aligned(1024))) char lds[WAVES * kRing * 2 * kBytes];
@@ -268,6 +268,19 @@ __global__ __launch_bounds__(WAVES * 64, 1) void packed_narrow_kernel(PackArgs a
     for (int w = 0; w < WAVES; ++w) top = fmaxf(top, ml[w * 32 + r][0]);
     const float weight = weight_of_state(m, top);
     float* const state = whole ? nullptr : state_of<D>(a, kvh, run, u == first_u ? 0 : 1);
+    constexpr uint32_t kItems = kTile * 8 / (WAVES * 64);  // of a thread: eight of a pair's 64 dims
+    uint32_t rows[kItems], cols[kItems];
+    Gate8 gates[DT / 2][kItems];
+#pragma unroll
+    for (uint32_t j = 0; j < kItems; ++j) {
+      const uint32_t i = tid + j * WAVES * 64;
+      pack_pair(a, tile, kvh, min(i / 8, pairs - 1), rows[j], cols[j]);
+      cols[j] = cols[j] * D + 8 * (i % 8);
+      if (whole && a.gate) {
+#pragma unroll
+        for (int g = 0; g < DT / 2; ++g) gates[g][j].load(a, rows[j], cols[j] + 64 * g);
+      }
+    }
 #pragma unroll
     for (int g = 0; g < DT / 2; ++g) {
       if (g) __syncthreads();
@@ -279,8 +292,10 @@ __global__ __launch_bounds__(WAVES * 64, 1) void packed_narrow_kernel(PackArgs a
         *(f4*)(to + ((2 * x + h) ^ (r & 15)) * 16) = f4{v[e], v[e + 1], v[e + 2], v[e + 3]} * weight;
       }
       __syncthreads();
-      for (uint32_t i = tid; i < pairs * 8; i += WAVES * 64) {  // eight dims of a pair
-        const uint32_t pair = i / 8, x = 2 * (i % 8);
+#pragma unroll
+      for (uint32_t j = 0; j < kItems; ++j) {
+        const uint32_t i = tid + j * WAVES * 64, pair = i / 8, x = 2 * (i % 8);
+        if (pair >= pairs) break;
         float pt = -INFINITY, lt = 0.f;
         f4 v0 = f4{0.f, 0.f, 0.f, 0.f}, v1 = v0;
 #pragma unroll
@@ -293,13 +308,12 @@ __global__ __launch_bounds__(WAVES * 64, 1) void packed_narrow_kernel(PackArgs a
           v0 += *(const f4*)(from + (x ^ (pair & 15)) * 16);
           v1 += *(const f4*)(from + ((x + 1) ^ (pair & 15)) * 16);
         }
-        const uint32_t dim = 64 * g + 8 * (i % 8);
         if (whole) {
-          pack_pair(a, tile, kvh, pair, row, head);
-          const bool sees = pack_seen(tile, row) != 0;
+          const bool sees = pack_seen(tile, rows[j]) != 0;
           const float inv = sees ? 1.0f / lt : 0.f;
-          store_pack8<BF16>(a, row, head * D + dim, v0 * inv, v1 * inv, sees);
+          store_pack8<BF16>(a, rows[j], cols[j] + 64 * g, v0 * inv, v1 * inv, gates[g][j], sees);
         } else {
+          const uint32_t dim = 64 * g + 8 * (i % 8);
           *(f4*)(state + pair * D + dim) = v0;
           *(f4*)(state + pair * D + dim + 4) = v1;
           if (dim == 0) *(f2*)(state + kTile * D + 2 * pair) = f2{pt, lt};
@@ -331,6 +345,10 @@ __global__ __launch_bounds__(512) void packed_merge_kernel(PackArgs a) {
   if (u1 > u0 && w0 == w1) return;  // written by the attention kernel itself
   const uint32_t item = tid % kItems, way = tid / kItems, d = 8 * (item % L);
   const uint32_t pr = min(kPairs * part + item / L, tile.pairs - 1);
+  uint32_t row, head;
+  pack_pair(a, tile, kvh, pr, row, head);
+  Gate8 gate;
+  if (a.gate) gate.load(a, row, head * D + d);
   f4 v0 = f4{0.f, 0.f, 0.f, 0.f}, v1 = v0;
   float top = -INFINITY, l = 0.f;
   auto add = [&](const f2& s, const f4& o0, const f4& o1) {
@@ -352,11 +370,9 @@ __global__ __launch_bounds__(512) void packed_merge_kernel(PackArgs a) {
   if (way != 0 || kPairs * part + item / L >= tile.pairs) return;
 #pragma unroll
   for (uint32_t j = 1; j < kWays; ++j) add(mls[j * kItems + item], acc0[j * kItems + item], acc1[j * kItems + item]);
-  uint32_t row, head;
-  pack_pair(a, tile, kvh, pr, row, head);
   const bool sees = pack_seen(tile, row) != 0;
   const float inv = sees ? 1.0f / l : 0.f;
-  store_pack8<BF16>(a, row, head * D + d, v0 * inv, v1 * inv, sees);
+  store_pack8<BF16>(a, row, head * D + d, v0 * inv, v1 * inv, gate, sees);
 }
 
 namespace {
@@ -381,10 +397,13 @@ hipError_t launch_packed_narrow(const PackArgs& a, uint32_t head_dim, bool bf16,
   return bf16 ? narrow_kernels<256, true>(a, s) : narrow_kernels<256, false>(a, s);
 }
 
-// Wide tiles once narrow ones would fill the device more than twice: 32 heads over 8 of 128, 603 causal rows (600 narrow tiles) 18 us
-// against 22, 400 rows 14 against 14, 4 x 128 rows behind 3,000 keys (512 tiles) 64 against 52; 16 over 4 of 256, 1,000 rows
-// (500) 52 against 38, 1,500 rows (748) 70 against 69, 8 x 200 rows (800) 26 against 47; 8 of 64, 2,000 rows (496) 28 against 24,
-// 4,000 rows (1,000) 54 against 81.
+// Wide tiles once narrow ones would fill the device more than twice (narrow against wide, us): 32 heads over 8 of 128, 4 x 128
+// rows behind 3,000 keys (512 tiles) 67 against 64, 4 x 200 (800 tiles) 120 against 65; 16 over 4 of 256, 1,000 rows (500) 33
+// against 42, 1,500 rows (748) 60 against 60, 8 x 200 rows (800) 37 against 16; 8 of 64, 2,000 rows (496) 25 against 29, 3,000
+// rows (744) 49 against 41. Where sequences are short a tile's fixed time weighs more, and a narrow one has a CU for itself:
+// beyond one for each CU 32 heads over 8 of 128, 400 rows (400) 14.6 against 13.7, 603 rows (600) 23 against 18; of 64, 603 rows
+// (600) 16 against 12, 8 of 64, 8 x 200 rows (400) 10.1 against 7.5; but 16 over 4 of 256, 603 rows (300) 22 against 28.
+// Narrow tiles of two waves, two of them on a CU, lose: 16 over 4 of 256, 603 rows 26, 8 of 64, 2,000 rows 34.
 // Runs, at the price of the deal and the merge, where narrow tiles leave half of the device idle over long sequences: one row, 32
 // heads over 8 of 128, 600 keys 10.9 us against 9.9, 4,096 keys 12 against 38; 16 over 4 of 256, 8 rows of up to 1,000 keys 24
 // against 21, one of 2,000 17 against 34; 200 rows behind 6,000 keys (100 tiles) 66 against 91; 32 over 8 of 128, 4 x 64 rows
@@ -395,7 +414,7 @@ PackPlan packed_plan(uint32_t q_rows, uint32_t seqs, uint32_t heads, uint32_t kv
   PackPlan p;
   const uint64_t pairs = (uint64_t)q_rows * (heads / kv_heads);
   const uint64_t full = pairs / kPackTile * kv_heads;  // narrow tiles that are surely full
-  p.wide = full >= (head_dim == 128 ? 9ull : 11ull) * cus / 4;
+  p.wide = full >= (head_dim == 128 ? 9ull : 11ull) * cus / 4 || (head_dim < 256 && max_k <= 1024 && full > cus);
   p.slots = (uint32_t)(pairs / (p.wide ? kPackWideTile : kPackTile) + seqs);
   const uint32_t least = head_dim == 256 ? 1024 : head_dim == 128 ? 768 : 1536;
   if (p.wide || p.slots > kPackSlots || max_k < least || full >= cus / 2 || kv_heads > cus / 2) return p;

@@ -8,12 +8,12 @@
 //     pair are in its two lanes, and the weights are, as they are, the operand of P^T: eight a lane for 16 keys, 4 h + j and
 //     8 + 4 h + j. V's operand is to hold the same keys for each dim: two transposing reads of four rows of V each.
 //   * K and V go into LDS by DMA, two blocks in turn, their chunks swizzled (packed_device.h). Two workgroups share a CU, and so
-//     two waves a SIMD, which need not be in step: 8,192 rows of 32 heads over 8 of 128 dims 517 us (1,060 TF); when it took
+//     two waves a SIMD, which need not be in step: 8,192 rows of 32 heads over 8 of 128 dims 522 us (1,050 TF); when it took
 //     585, eight waves in one workgroup on a ring of four blocks took 611, and with the two of a SIMD kept half a block apart
 //     614; three workgroups with blocks of 32 keys 620. Matrix and vector instructions (the softmax) bound it, 45 and 42 %
 //     of the cycles, and they hardly overlap.
 //   * The softmax's reference point moves only where a score exceeds it by 2^8, so O is rarely rescaled.
-//   * Of 256 dims, 24 prompts of up to 2,307 rows and 16 heads over 4, 19.5 k rows in all, with gates: 400 us; there the bytes of
+//   * Of 256 dims, 24 prompts of up to 2,307 rows and 16 heads over 4, 19.5 k rows in all, with gates: 395 us; there the bytes of
 //     Q, y and the gates alone are 161 us.
 //   * Keys past the sequence's end are its last one again, masked: another sequence's values are never touched.
 #include "packed_device.h"
@@ -207,11 +207,28 @@ __global__ __launch_bounds__(256, 2) void packed_wide_kernel(PackArgs a) {
 
   // Through LDS, 64 dims at a time, so that rows are written and gates read in whole lines. Four dims of pair r at chunk x
   // lie at x ^ r % 16.
+  // The gates of the next 64 dims are read meanwhile.
   l = sum_of_halves(l);
   const float inv = seen ? 1.0f / l : 0.f;  // (a row that sees nothing is zero; one that sees only -infinity is NaN)
   char* const mine = lds + wave * 8192;
+  auto at = [&](int k, uint32_t& row, uint32_t& col) {  // pair 8 k + lane / 8, dims 8 (lane % 8) .. + 7
+    const uint32_t pair = 32 * wave + 8 * k + lane / 8;
+    pack_pair(a, tile, kvh, min(pair, tile.pairs - 1), row, col);
+    col = col * D + 8 * (lane % 8);
+    return pair < tile.pairs;
+  };
+  Gate8 gates[2][4];
+  auto read_gates = [&](int g) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t row, col;
+      if (at(k, row, col)) gates[g % 2][k].load(a, row, col + 64 * g);
+    }
+  };
+  if (a.gate) read_gates(0);
 #pragma unroll
   for (int g = 0; g < DT / 2; ++g) {
+    if (a.gate && g + 1 < DT / 2) read_gates(g + 1);
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
       const f16v& v = o[2 * g + x / 4];
@@ -225,9 +242,8 @@ __global__ __launch_bounds__(256, 2) void packed_wide_kernel(PackArgs a) {
       const uint32_t pair = 8 * k + lane / 8, x = 2 * (lane % 8);
       const f4 v0 = *(const f4*)(mine + pair * 256 + ((x ^ (pair & 15)) * 16));
       const f4 v1 = *(const f4*)(mine + pair * 256 + (((x + 1) ^ (pair & 15)) * 16));
-      if (32 * wave + pair >= tile.pairs) continue;
-      pack_pair(a, tile, kvh, 32 * wave + pair, row, head);
-      store_pack8<BF16>(a, row, head * D + 64 * g + 8 * (lane % 8), v0, v1, pack_seen(tile, row) != 0);
+      uint32_t row, col;
+      if (at(k, row, col)) store_pack8<BF16>(a, row, col + 64 * g, v0, v1, gates[g % 2][k], pack_seen(tile, row) != 0);
     }
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
