@@ -148,7 +148,8 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void fp8_gemm_kernel(Fp8GemmArgs a
   const uint32_t wm = wave / WN, wn = wave % WN, r = lane & 31, h = lane >> 5;
 
   // A DMA fetches 8 rows of 128 bytes, from[i] on, the wave's i-th of X's and then of W's; rows past the end are the last one
-  // again.
+  // again. most[i]: how far the last of the eight lies from the first, at most 7 x 2^23 bytes (all the rows behind the first may
+  // span more than 2^32).
   constexpr int kXPieces = BM / 8 / NW;
   static_assert(kXPieces * 8 * NW == BM && NW % 2 == 0, "a wave's DMAs are X's or W's as their number says");
   const uint8_t* from[kPieces];
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(WM * WN * 64, 1) void fp8_gemm_kernel(Fp8GemmArgs a
       const uint32_t last = of_x ? a.m - 1 - m0 : a.n - 1 - n0, ld = of_x ? a.ldx : a.ldw;
       const uint32_t first = min(((of_x ? i : i - kXPieces) * NW + wave) * 8, last);
       from[i] = (of_x ? a.x + (size_t)m0 * ld : a.w + (size_t)n0 * ld) + (size_t)first * ld;
-      most[i] = (last - first) * ld;
+      most[i] = min(last - first, 7u) * ld;
     }
   };
   const uint32_t xlane = lane / 8 * a.ldx, wlane = lane / 8 * a.ldw, chunk = ((lane & 7) ^ row_key(8 * wave + lane / 8)) * 16;

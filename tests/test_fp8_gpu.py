@@ -397,6 +397,34 @@ def test_rows_past_4_gib(gpu, kernels, stream):
     wd.free()
 
 
+@pytest.mark.parametrize("rows,of_w", [(515, False), (601, False), (607, False), (601, True), (607, True)])
+@pytest.mark.parametrize("epi", [Epilogue.StoreF32, Epilogue.StoreF16])
+def test_an_odd_number_of_rows_past_4_gib(gpu, kernels, stream, rows, of_w, epi):
+    """X's, or W's, rows 2^23 bytes apart and not a multiple of eight of them: from some row the distance to the last one, in
+    bytes, is small again modulo 2^32. Small whole numbers, exact."""
+    from decide_amd.hip import DeviceArray
+
+    few, k, ld = 40, 200, 1 << 23
+    m, n = (few, rows) if of_w else (rows, few)
+    p = Product(m, n, k, codes=lambda rng, shape: rng.integers(-8, 9, shape).astype(np.float64))
+    big = DeviceArray((rows * ld,), np.uint8)
+    far, near = (p.w, p.x) if of_w else (p.x, p.w)
+    for r in range(rows):
+        row = np.ascontiguousarray(far[r])
+        check(rt().hipMemcpy(big.ptr + r * ld, row.ctypes.data, row.nbytes, 1), "copy")
+    nd, sx, sw = to_dev(near), to_dev(ref.scale_bytes(p.ex, up(m, 4))), to_dev(ref.scale_bytes(p.ew, up(len(p.ew), 4)))
+    x, w = ((nd, 0), (big, 0)) if of_w else ((big, 0), (nd, 0))
+    lds = [near.shape[1], ld] if of_w else [ld, near.shape[1]]
+    y = full((m, up(n, 4)), np.float32 if epi == Epilogue.StoreF32 else np.float16, 0)
+    kernels.fp8.gemm(stream, Fp8Matrix(x, lds[0], (sx, 0), up(m, 4)), Fp8Matrix(w, lds[1], (sw, 0), up(len(p.ew), 4)), (y, 0),
+                     up(n, 4), m, n, k, epi)
+    sync()
+    got = to_host(y)[:, :n]
+    big.free()
+    with np.errstate(over="ignore"):
+        assert np.array_equal(got, p.want().astype(got.dtype))
+
+
 def test_warm_up_loads_the_8_bit_kernels(gpu, stream):
     k = Kernels()
     k.gemm.warm_up(stream, 64)
