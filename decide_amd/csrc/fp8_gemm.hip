@@ -424,10 +424,10 @@ Fp8Plan fp8_gemm_plan_of(int v, uint32_t splits, uint32_t m, uint32_t n, uint32_
   p.variant = v;
   p.mtiles = (m + kVariants[v].bm - 1) / kVariants[v].bm;
   p.ntiles = (n + kVariants[v].bn - 1) / kVariants[v].bn;
-  const uint32_t words = (k + kFp8Word - 1) / kFp8Word;
-  const uint32_t each = (words + splits - 1) / std::max(1u, splits);
-  p.kps = std::max(1u, each) * kFp8Word;
-  p.splits = std::max(1u, (words + each - 1) / std::max(1u, each));
+  const uint32_t words = std::max(1u, (k + kFp8Word - 1) / kFp8Word);  // no columns: one part, of none
+  const uint32_t each = (words + splits - 1) / splits;
+  p.kps = each * kFp8Word;
+  p.splits = (words + each - 1) / each;
   if (p.splits > 1) p.ws_bytes = (uint64_t)p.splits * m * ((n + 3) / 4 * 4) * sizeof(float);
   return p;
 }

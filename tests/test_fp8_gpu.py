@@ -305,6 +305,27 @@ def test_all_scales_are_followed(gpu, kernels, stream):
             assert np.array_equal(got, want.astype(t).astype(np.float64)), (epi, ex, ew)
 
 
+@pytest.mark.parametrize("m,n", [(1, 32), (17, 64), (300, 96), (1100, 4128)])
+def test_no_columns_sum_to_zero(gpu, kernels, stream, m, n):
+    """K = 0, with codes, scales or neither: zeros are stored, nothing is added, SwiGLU of zeros is zero, as dh_gemm_nt's."""
+    some = full((4096,), np.uint8, 0x7f)
+    lds = max(up(m, 4), up(up(n, 128) // 128, 4))
+    nt_x, nt_w = full((m, 8), np.float16, np.nan), full((n, 8), np.float16, np.nan)
+    kernels.fp8.gemm_ws(stream, m, n, 0)
+    for x in (Fp8Matrix((some, 0), 0, (some, 0), lds), Fp8Matrix((0, 0), 0, (0, 0), lds), Fp8Matrix((0, 0), 128, (0, 0), lds)):
+        for epi in Epilogue:
+            wide, f32 = n // 2 if epi == Epilogue.SwigluF16 else n, epi in (Epilogue.StoreF32, Epilogue.AddF32)
+            before = np.random.default_rng(m).standard_normal((m + 1, wide + 4)).astype(np.float32 if f32 else np.float16)
+            yd, nt = to_dev(before), to_dev(before)
+            kernels.fp8.gemm(stream, x, x, (yd, 0), wide + 4, m, n, 0, epi)
+            kernels.gemm.gemm(stream, (nt_x, 0), (nt_w, 0), (nt, 0), m, n, 0, 8, 8, wide + 4, epi)
+            sync()
+            want = before.copy()
+            if epi != Epilogue.AddF32:
+                want[:m, :wide] = 0
+            assert np.array_equal(to_host(yd), want) and np.array_equal(to_host(nt), want)
+
+
 def test_a_row_has_the_same_bits_wherever_it_stands(gpu, kernels, stream):
     p = Product(300, 96, 1030)
     p.x[:], p.ex[:] = p.x[0], p.ex[0]
