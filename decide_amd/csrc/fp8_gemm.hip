@@ -420,15 +420,16 @@ void launch(const Fp8GemmArgs& a, uint32_t grid, hipStream_t s) {
 int fp8_variant_count() { return kVariantCount; }
 
 Fp8Plan fp8_gemm_plan_of(int v, uint32_t splits, uint32_t m, uint32_t n, uint32_t k) {
+  auto parts = [](uint32_t x, uint32_t of) { return (uint32_t)(((uint64_t)x + of - 1) / of); };  // (x may end at 2^32 - 1)
   Fp8Plan p;
   p.variant = v;
-  p.mtiles = (m + kVariants[v].bm - 1) / kVariants[v].bm;
-  p.ntiles = (n + kVariants[v].bn - 1) / kVariants[v].bn;
-  const uint32_t words = std::max(1u, (k + kFp8Word - 1) / kFp8Word);  // no columns: one part, of none
-  const uint32_t each = (words + splits - 1) / splits;
+  p.mtiles = parts(m, kVariants[v].bm);
+  p.ntiles = parts(n, kVariants[v].bn);
+  const uint32_t words = std::max(1u, parts(k, kFp8Word));  // no columns: one part, of none
+  const uint32_t each = parts(words, splits);
   p.kps = each * kFp8Word;
-  p.splits = (words + each - 1) / each;
-  if (p.splits > 1) p.ws_bytes = (uint64_t)p.splits * m * ((n + 3) / 4 * 4) * sizeof(float);
+  p.splits = parts(words, each);
+  if (p.splits > 1) p.ws_bytes = (uint64_t)p.splits * m * (((uint64_t)n + 3) / 4 * 4) * sizeof(float);
   return p;
 }
 

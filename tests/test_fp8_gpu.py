@@ -326,6 +326,18 @@ def test_no_columns_sum_to_zero(gpu, kernels, stream, m, n):
             assert np.array_equal(to_host(yd), want) and np.array_equal(to_host(nt), want)
 
 
+@pytest.mark.parametrize("n", [(1 << 32) - 4, (1 << 32) - 32, (1 << 32) - 256, 1 << 31])
+def test_more_columns_than_a_launch_takes_are_refused(gpu, kernels, stream, n):
+    d = full((64,), np.uint8, 7)
+    for epi, ldy in ((Epilogue.StoreF32, n), (Epilogue.SwigluF16, n // 2)):
+        if epi == Epilogue.StoreF32 or n % 32 == 0:
+            m = Fp8Matrix((d, 0), 0, (d, 0), 1 << 26)
+            with pytest.raises(AssertionError, match="exceed one launch"):
+                kernels.fp8.gemm(stream, m, m, (d, 0), ldy, 1, n, 0, epi)
+    sync()
+    assert (to_host(d) == 7).all()
+
+
 def test_a_row_has_the_same_bits_wherever_it_stands(gpu, kernels, stream):
     p = Product(300, 96, 1030)
     p.x[:], p.ex[:] = p.x[0], p.ex[0]

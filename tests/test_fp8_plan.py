@@ -44,3 +44,15 @@ def test_parts_cover_the_columns_and_none_is_empty(m, n, k, epi):
     p = plan(m, n, k, epi)
     assert p.kps % WORD == 0 and (p.splits - 1) * p.kps < k <= p.splits * p.kps
     assert p.ws_bytes == (p.splits * m * n * 4 if p.splits > 1 else 0)
+
+
+@pytest.mark.parametrize("epi", [Epilogue.StoreF32, Epilogue.StoreF16])
+@pytest.mark.parametrize("n", [(1 << 32) - 1, (1 << 32) - 4, (1 << 32) - 127, (1 << 32) - 255])
+@pytest.mark.parametrize("k", [0, 128, 9216])
+def test_columns_up_to_the_last_of_32_bits_are_counted(n, k, epi):
+    """Rounding n up to whole tiles passes 32 bits; the caller's limit of one launch counts the tiles."""
+    for v, columns in ((0, 256), (1, 128), (2, 128)):
+        p = plan_of(v, 1, 1, n, k)
+        assert p.ntiles == -(-n // columns) and p.mtiles == 1
+    p = plan(1, n, k, epi)
+    assert p.ntiles >= 1 << 24 and p.splits == 1
