@@ -16,6 +16,10 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
 constexpr float kPackLazy = 8.0f;  // log2 headroom of the softmax's reference point (weights up to 256)
 constexpr float kPackLog2e = 1.4426950408889634f;
+// A weight is 2^(score c - m) with the product unrounded, while the reference point m is the largest one's rounded: half a step
+// of m apart. From |m| = 2^20 on, where that is 2^-4 and grows with m until weights overflow, a pair's products are rounded too,
+// so that the largest weighs 2^0 again.
+constexpr float kPackFar = 0x1p20f;
 
 // fp16 or bf16, eight to an operand
 template <bool BF16>
@@ -96,6 +100,18 @@ __device__ __forceinline__ uint32_t max_of_wave(uint32_t v) {
 // weight of a state whose reference point is m among those whose largest is top; none where it met no score
 __device__ __forceinline__ float weight_of_state(float m, float top) {
   return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+}
+// For a pair whose reference point is `m`: rounds the products where it lies far out; returns what is left of the factor c.
+template <int N>
+__device__ __forceinline__ float round_far(f16v* st, float c, float m) {
+  if (!__any(fabsf(m) >= kPackFar)) return c;
+  const bool far = fabsf(m) >= kPackFar;
+  const float f = far ? c : 1.0f;  // (the tile's other pairs keep their bits)
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) st[t][e] *= f;
+  return far ? 1.0f : c;
 }
 __device__ __forceinline__ float sigmoid_of(float x) { return 1.0f / (1.0f + __expf(-x)); }
 

@@ -200,22 +200,22 @@ __global__ __launch_bounds__(WAVES * 64, 1) void packed_narrow_kernel(PackArgs a
 #pragma unroll
       for (int e = 1; e < 16; ++e) top = fmaxf(top, st[e]);
       top = max_of_halves(top) * c;
-      if (__any(top > m + kPackLazy)) {
-        const float mnew = top > m + kPackLazy ? top : m;  // a pair's own: the others of the tile keep their bits
+      if (__any(top - m > kPackLazy)) {
+        const float mnew = top - m > kPackLazy ? top : m;  // a pair's own: the others of the tile keep their bits
         const float alpha = weight_of_state(m, mnew);
         l *= alpha;
         m = mnew;
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[i] *= alpha;
       }
-      const float mref = m == -INFINITY ? 0.f : m;
+      const float mref = m == -INFINITY ? 0.f : m, factor = round_far<1>(&st, c, mref);
       s8 p[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         float w[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          w[e] = __builtin_amdgcn_exp2f(fmaf(st[8 * x + e], c, -mref));
+          w[e] = __builtin_amdgcn_exp2f(fmaf(st[8 * x + e], factor, -mref));
           l += w[e];
         }
         p[x] = pack8<BF16>(w);

@@ -134,21 +134,21 @@ __global__ __launch_bounds__(256, 2) void packed_wide_kernel(PackArgs a) {
 #pragma unroll
       for (int e = 1; e < 16 * T; ++e) top = fmaxf(top, st[e / 16][e % 16]);
       top = max_of_halves(top) * c;
-      if (__any(top > m + kPackLazy)) {
-        const float mnew = top > m + kPackLazy ? top : m;  // a pair's own: the others of the tile keep their bits
+      if (__any(top - m > kPackLazy)) {
+        const float mnew = top - m > kPackLazy ? top : m;  // a pair's own: the others of the tile keep their bits
         const float alpha = weight_of_state(m, mnew);
         l *= alpha;
         m = mnew;
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[i] *= alpha;
       }
-      const float mref = m == -INFINITY ? 0.f : m;
+      const float mref = m == -INFINITY ? 0.f : m, factor = round_far<T>(st, c, mref);
 #pragma unroll
       for (int x = 0; x < 2 * T; ++x) {
         float w[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          w[e] = __builtin_amdgcn_exp2f(fmaf(st[x / 2][8 * (x % 2) + e], c, -mref));
+          w[e] = __builtin_amdgcn_exp2f(fmaf(st[x / 2][8 * (x % 2) + e], factor, -mref));
           l += w[e];
         }
         p[x] = pack8<BF16>(w);

@@ -183,6 +183,58 @@ def test_scales_and_sharp_weights(gpu, kernels, stream, nq, nk, scale, size):
         Packed(nq, nk, 4, 2, dim, dtype, scale=scale, size=size).check(kernels, stream)
 
 
+FAR = [(4, 2, [100], [100]), (4, 1, [3], [2000]), (4, 2, [5, 1], [5, 1]), (64, 2, [400], [400])]  # narrow tiles, runs, wide tiles
+
+
+def winners_mean(p, winner):
+    """What rows are whose seen keys t with winner(t) weigh the same and the others nothing: the mean of their values. The weights
+    are 1 exactly; `seen` additions of them and of their values are off by 2 U each at most, in numerator and denominator."""
+    want, err = np.full((2, p.rows, p.heads, p.dim), np.nan)
+    for s in range(len(p.q0) - 1):
+        for i in range(p.q0[s], p.q0[s + 1]):
+            n = p.k0[s + 1] - p.k0[s] - (p.q0[s + 1] - 1 - i)
+            v = p.v[p.k0[s] + np.flatnonzero(winner(np.arange(n)))]
+            want[i] = np.repeat(v.mean(0), p.heads // p.kv, 0)
+            err[i] = (4 * n + 8) * 2.0 ** -24 * np.repeat(np.abs(v).mean(0), p.heads // p.kv, 0)
+    err = err * (1 + HALF[p.dtype]) + HALF[p.dtype] * np.abs(want) + 2.0 ** -25
+    rows = slice(p.q0[0], p.q0[-1])
+    return want.reshape(p.rows, -1)[rows], err.reshape(p.rows, -1)[rows]
+
+
+@pytest.mark.parametrize("scale", [300.0, 1e5, 1e25])
+@pytest.mark.parametrize("dim,dtype", [(64, "bf16"), (128, "f16"), (256, "bf16"), (256, "f16")])
+@pytest.mark.parametrize("heads,kv,nq,nk", FAR)
+def test_scores_far_from_zero_weigh_as_others_do(gpu, kernels, stream, dim, dtype, heads, kv, nq, nk, scale):
+    """Scores of 2^22.6 times the scale, whose fp32 steps are 2^6 and more: every third key has the largest, or all have the same."""
+    for sign, step in ((1.0, 3), (-1.0, 1)):
+        p = Packed(nq, nk, heads, kv, dim, dtype, gate=False, scale=scale)
+        p.q[:], p.k[:] = 0.0, 0.0
+        p.q[..., 3] = 127.0  # (odd: a power of two's product with the scale has no rounding)
+        for s in range(len(nq)):
+            t = np.arange(nk[s])
+            p.k[p.k0[s]:p.k0[s + 1], :, 3] = (sign * np.where(t % step == 0, 201 * 2.0 ** 8, 200 * 2.0 ** 8))[:, None]
+        p.qr, p.kr = to_type(p.q, dtype)[0], to_type(p.k, dtype)[0]
+        got = p.run(kernels, stream)[p.q0[0]:p.q0[-1]]
+        want, err = winners_mean(p, lambda t: t % step == 0)
+        assert (np.abs(got - want) <= err).all()
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, "f16"), (128, "bf16"), (256, "f16")])
+@pytest.mark.parametrize("heads,kv,nq,nk", FAR)
+def test_scores_far_from_zero_leave_other_rows_alone(gpu, kernels, stream, dim, dtype, heads, kv, nq, nk):
+    """Every other row's scores are about 2^29; the rows between are, to the bit, as they are among rows like themselves."""
+    clean, far = (Packed(nq, nk, heads, kv, dim, dtype, scale=0.9, size=0.5) for _ in range(2))
+    for p in (clean, far):
+        p.q[..., 3] = 0.0
+        p.k[..., 3] = 201 * 2.0 ** 7
+    far.q[1::2, :, 3] = 203 * 2.0 ** 7
+    for p in (clean, far):
+        p.qr, p.kr = to_type(p.q, dtype)[0], to_type(p.k, dtype)[0]
+    a, b = clean.run(kernels, stream), far.run(kernels, stream)
+    rows = np.arange(far.q0[0], far.q0[-1])
+    assert np.array_equal(a[rows[rows % 2 == 0]], b[rows[rows % 2 == 0]]) and np.isfinite(b[rows]).all()
+
+
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("nq,nk", [([90, 90, 90], [90, 90, 90]), ([1, 1, 1], [500, 700, 300])])
 def test_what_is_not_finite_stays_in_its_sequence(gpu, kernels, stream, dim, nq, nk):
