@@ -46,8 +46,8 @@ __device__ __forceinline__ s8 pack8(const float* v) {
 }
 
 // What a scale leaves to be done to Q: a negative one's sign goes to it, so that the largest score is the largest product; and
-// so does zero (or what is next to it and would be zero as fp32), which would make NaN of a masked score's -infinity. Returns
-// the factor of the exponent.
+// so does zero, which would make NaN of a masked score's -infinity. Returns the factor of the exponent, a subnormal one among
+// them: bf16's products reach 2^128.
 template <bool BF16, int N>
 __device__ __forceinline__ float scale_into(s8 (&q)[N], float scale) {
   const float c = fabsf(scale) * kPackLog2e;
@@ -55,7 +55,7 @@ __device__ __forceinline__ float scale_into(s8 (&q)[N], float scale) {
 #pragma unroll
     for (int x = 0; x < N; ++x) q[x] ^= (short)0x8000;
   }
-  if (c >= 0x1p-126f) return c;
+  if (c > 0.f) return c;
   constexpr short kExp = BF16 ? 0x7f80 : 0x7c00;
 #pragma unroll
   for (int x = 0; x < N; ++x) {

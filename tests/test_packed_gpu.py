@@ -186,6 +186,15 @@ def test_scales_and_sharp_weights(gpu, kernels, stream, nq, nk, scale, size):
 FAR = [(4, 2, [100], [100]), (4, 1, [3], [2000]), (4, 2, [5, 1], [5, 1]), (64, 2, [400], [400])]  # narrow tiles, runs, wide tiles
 
 
+@pytest.mark.parametrize("scale", [2.0 ** -127, -(2.0 ** -128), 2.0 ** -149, 0.0])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv,nq,nk", FAR)
+def test_scales_below_the_normal_numbers(gpu, kernels, stream, dim, heads, kv, nq, nk, scale):
+    """bf16's products of 2^124 and such a scale: scores of about 1/8. The factor of the exponent is rounded to a multiple of 2^-149,
+    which moves no score by more than 2^-22, within the 2^-20 that the bound leaves."""
+    Packed(nq, nk, heads, kv, dim, "bf16", scale=scale, size=2.0 ** 60).check(kernels, stream)
+
+
 def winners_mean(p, winner):
     """What rows are whose seen keys t with winner(t) weigh the same and the others nothing: the mean of their values. The weights
     are 1 exactly; `seen` additions of them and of their values are off by 2 U each at most, in numerator and denominator."""
