@@ -47,7 +47,7 @@ int dh_attention_packed(dh_ctx* ctx, void* stream, const dh_packed_batch* batch,
   int rc = check_shape(op, batch->q_rows, batch->seqs, heads, kv_heads, head_dim);
   if (rc != DH_OK) return rc;
   if (dtype > 1) return fail(DH_EINVAL, "%s: dtype %u is not one of 0 (fp16), 1 (bf16)", op, dtype);
-  if (!std::isfinite(scale)) return fail(DH_EINVAL, "%s: scale must be finite", op);
+  if (!(std::fabs(scale) <= 0x1p127f)) return fail(DH_EINVAL, "%s: scale must be finite and at most 2^127", op);
   const uint64_t wide = (uint64_t)heads * head_dim, narrow = (uint64_t)kv_heads * head_dim;
   rc = check_rows(op, "q", q, ldq, 8, wide, 16);
   if (rc == DH_OK) rc = check_rows(op, "k", k, ldk, 8, narrow, 16);

@@ -779,7 +779,7 @@ typedef struct dh_packed_batch {
  * on keys and values that it does not see, whatever they hold; what it sees is
  * followed through softmax, infinities and NaN among it.
  * Contract: head_dim 64, 128 or 256; heads % kv_heads == 0, at most 1,024 heads
- * a kv head; scale finite; ldq, ldk, ldv % 8 == 0, ldy, ldg % 4 == 0, each
+ * a kv head; |scale| at most 2^127; ldq, ldk, ldv % 8 == 0, ldy, ldg % 4 == 0, each
  * covering its heads; q, k, v and gate 16-byte, y 8-byte aligned. Few rows over
  * many keys are divided across workgroups and merged through the context's
  * forward-kernel workspace (dh_attention_packed_ws; an eager call of the same

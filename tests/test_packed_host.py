@@ -97,6 +97,14 @@ def test_packed_attention_refuses(kw, msg):
     _refused(_attn(**kw), msg)
 
 
+@pytest.mark.parametrize("scale", [1.8e38, -1.8e38, 3.4e38, -3.4e38, float("nan"), float("-inf")])
+def test_scales_past_2_to_the_127_are_refused(scale):
+    """Times log2(e), by which the exponents are taken, they would be infinite."""
+    _refused(_attn(scale=scale), "scale")
+    for fine in (2.0 ** 127, -(2.0 ** 127), 2.0 ** -149, 0.0):
+        _refused(_attn(scale=fine), "null context")
+
+
 def test_scale_strides_past_their_addressing_are_refused():
     wide = dict(lds=(1 << 26) + 4)
     _refused(_rows(out=wide), "exceeds 2^26")
