@@ -777,7 +777,11 @@ typedef struct dh_packed_batch {
  * elements. Scores and softmax fp32; a weight relative to its row's largest is
  * rounded to dtype as the operand of its product with v. A row does not depend
  * on keys and values that it does not see, whatever they hold; what it sees is
- * followed through softmax, infinities and NaN among it.
+ * followed through softmax, infinities and NaN among it. Two limits: an infinite
+ * value of a key whose weight is too small for dtype makes its column infinite
+ * or NaN (zero times infinity), as the call's layout has it; and values are
+ * summed in fp32 with weights of up to 2^8 before they are divided by the
+ * weights' sum, so that bfloat16 values near 2^127 can give infinity.
  * Contract: head_dim 64, 128 or 256; heads % kv_heads == 0, at most 1,024 heads
  * a kv head; |scale| at most 2^127; ldq, ldk, ldv % 8 == 0, ldy, ldg % 4 == 0, each
  * covering its heads; q, k, v and gate 16-byte, y 8-byte aligned. Few rows over

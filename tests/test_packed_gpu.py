@@ -309,6 +309,33 @@ def test_values_that_a_row_does_not_see_may_be_anything(gpu, kernels, stream, di
     assert np.array_equal(got[rows], want[rows], equal_nan=True)
 
 
+@pytest.mark.parametrize("dim,dtype", [(64, "f16"), (128, "bf16"), (256, "f16")])
+@pytest.mark.parametrize("heads,kv,nq,nk", HIDDEN)
+def test_infinite_values_of_keys_that_weigh_next_to_nothing(gpu, kernels, stream, dim, dtype, heads, kv, nq, nk):
+    """Sharp weights, many of them zero as an operand, and infinite values: the first key's and another's that every row sees if it
+    sees any, and the last two keys'. Their columns are infinite or NaN in the rows that see them, never finite; all else is as it
+    would be without, to the bit."""
+    clean, bad = (Packed(nq, nk, heads, kv, dim, dtype, size=3.0) for _ in range(2))
+    want = clean.run(kernels, stream)
+    marks = np.zeros((2, bad.keys, kv, dim), bool)  # +infinity, -infinity
+    for s in range(len(nq)):
+        k0, k1 = int(bad.k0[s]), int(bad.k0[s + 1])
+        for key, col, what in ((k0, 5, 0), (k0 + max(nk[s] - nq[s], 0), dim - 1, 1), (k1 - 1, 7, 0), (k1 - 2, 40, 1)):
+            marks[what, key, :, col] = True
+    for what, value in enumerate((np.inf, -np.inf)):
+        bad.vr[marks[what]] = to_type(np.full(1, value), dtype)[0][0]
+    got = bad.run(kernels, stream)
+    seen = np.zeros((2, bad.rows, heads, dim), bool)
+    for s in range(len(nq)):
+        for i in range(nq[s]):
+            n = max(nk[s] - nq[s] + i + 1, 0)
+            seen[:, bad.q0[s] + i] = np.repeat(marks[:, bad.k0[s]:bad.k0[s] + n].any(1), heads // kv, 1)
+    plus, minus = seen.reshape(2, bad.rows, -1)[:, bad.q0[0]:bad.q0[-1]]
+    got, want = got[bad.q0[0]:bad.q0[-1]], want[bad.q0[0]:bad.q0[-1]]
+    assert (np.isnan(got[plus]) | (got[plus] == np.inf)).all() and (np.isnan(got[minus]) | (got[minus] == -np.inf)).all()
+    assert np.array_equal(got[~(plus | minus)], want[~(plus | minus)]) and np.isfinite(got[~(plus | minus)]).all()
+
+
 def test_rows_that_see_nothing_are_zero_whatever_they_hold(gpu, kernels, stream):
     for dim in (64, 128, 256):
         p = Packed([9, 300], [4, 0], 4, 2, dim, "bf16")
