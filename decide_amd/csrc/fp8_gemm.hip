@@ -8,8 +8,9 @@
 //     ends 13 bits below the largest, cutting what lies lower towards zero; only these sums of eight meet in fp32. Measured
 //     against 64 bits: 1.5e-5 of the result (2-norm) on normal operands, 4e-5 where columns differ by a factor of e. Rounding
 //     to fp16 costs 2.1e-4.
-//   * fp32 outputs: the codes times their scales as bf16, which holds them exactly, on v_mfma_f32_32x32x16_bf16 at half the
-//     rate, whose sums are fp32's: 2e-7. (The 8-bit instruction without scales cuts just the same.)
+//   * fp32 outputs: the codes times their scales as bf16, which holds them exactly where the scale's byte is 3 .. 246 (448 x 2^119
+//     down to 2^-9 x 2^-124, bf16's smallest), on v_mfma_f32_32x32x16_bf16 at half the rate, whose sums are fp32's: 2e-7. (The
+//     8-bit instruction without scales cuts just the same.)
 //   * W is the first operand, so that a lane gets one row of y and four columns at a time, in four groups.
 //   * K runs in stages of 128 columns, whole cache lines, through a ring of NBUF buffers in LDS, filled by DMA. Each half of a
 //     stage is read into registers while the products of the half before it run, so a stage's buffer is free for another
@@ -67,7 +68,7 @@ __device__ __forceinline__ void dma4(uint32_t m0, uint32_t voff, const void* sba
 }
 #pragma clang diagnostic pop
 
-// Eight codes times their scale, exactly.
+// Eight codes times their scale, exactly within bf16's range.
 __device__ __forceinline__ b8 widened(uint32_t lo, uint32_t hi, float scale) {
   const b2 p[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false),
                    __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true),

@@ -734,6 +734,11 @@ int dh_fp8_quant_blocks(dh_ctx* ctx, void* stream, const void* w, uint32_t ldw, 
  * neighbouring columns are first added by the matrix instruction, which cuts
  * what lies more than 13 bits below the largest of them (2^-13 of the largest
  * product a term at most, a thirtieth of an fp16 rounding on ordinary data).
+ * With fp32 outputs values are held as bfloat16 first: exactly where the byte
+ * of their scale is 3 .. 246, whatever the code; beyond, what is past
+ * bfloat16's largest number counts as infinite and what is no multiple of its
+ * smallest, 2^-133, is rounded to one. (The functions above bring only values
+ * of 1.9375 x 2^127 and more there, whose code times scale is 2^128.)
  * Contract: any m, n and k (n % 32 == 0 for SwiGLU); ldy % 4 == 0; y 16-byte
  * (fp32 outputs) or 8-byte (fp16 outputs) aligned; a code of NaN makes its row
  * (of x) or column (of w's row) NaN. Where there are few tiles K is divided and

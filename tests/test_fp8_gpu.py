@@ -305,6 +305,37 @@ def test_all_scales_are_followed(gpu, kernels, stream):
             assert np.array_equal(got, want.astype(t).astype(np.float64)), (epi, ex, ew)
 
 
+@pytest.mark.parametrize("value", [448.0, 2.0 ** -9])
+@pytest.mark.parametrize("m,n", [(66, 300), (300, 260), (1100, 4100)])
+@pytest.mark.parametrize("epi,ends", [(Epilogue.StoreF32, (119, -124)), (Epilogue.StoreF16, (127, -126))])
+def test_the_ends_of_the_scales_are_followed(gpu, kernels, stream, m, n, epi, ends, value):
+    """The largest and the smallest code at the largest and the smallest scale that all codes are exact with, as x's and as w's;
+    the others are of 1 and the inverse scale. Few terms, sums exact."""
+    for e in ends:
+        for of_x in (True, False):
+            p = Product(m, n, 320, codes=lambda rng, s: np.where(rng.random(s) < 0.1, rng.choice([-1.0, 1.0], s), 0.0))
+            far, near = (p.x, p.w) if of_x else (p.w, p.x)
+            far[(far & 0x7f) == 0x38] += ref.encode(value) - 0x38  # (the sign stays)
+            (p.ex if of_x else p.ew)[:], (p.ew if of_x else p.ex)[:] = e, max(-e, -126)
+            want, got = p.want(), p.run(kernels, stream, epi)
+            assert np.abs(want).max() >= value and np.array_equal(got, want), (e, of_x)
+
+
+def test_coded_values_past_bfloat16_are_infinite_with_fp32_outputs(gpu, kernels, stream):
+    """fp32's largest value is coded as 256 x 2^120: times 2^-120 finite in an fp16 output. The largest that is coded within
+    bfloat16's range is finite in both."""
+    x = np.zeros((2, 128), np.float64)
+    x[0, 0], x[1, 0] = np.float32(3.4028235e38), np.float32(1.93 * 2.0 ** 127)
+    p = Product(2, 32, 128)
+    p.x, p.ex = ref.quant(x, 1)
+    p.w, p.ew = ref.encode(np.ones((32, 128))), np.full((1, 1), -120)
+    want = p.want()
+    assert (want[:, 0] == (256, 240)).all() and (p.ex == 120).all()
+    assert np.array_equal(p.run(kernels, stream, Epilogue.StoreF16), want)
+    got = p.run(kernels, stream, Epilogue.StoreF32)
+    assert np.isinf(got[0]).all() and np.array_equal(got[1], want[1])
+
+
 @pytest.mark.parametrize("m,n", [(1, 32), (17, 64), (300, 96), (1100, 4128)])
 def test_no_columns_sum_to_zero(gpu, kernels, stream, m, n):
     """K = 0, with codes, scales or neither: zeros are stored, nothing is added, SwiGLU of zeros is zero, as dh_gemm_nt's."""
