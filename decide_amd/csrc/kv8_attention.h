@@ -272,6 +272,19 @@ __device__ __forceinline__ void mask_scores(V& s, float cs, uint32_t mine, float
   unit = mine != 0 && cs > 0.f ? cs : 1.0f;
 }
 
+// A weight is 2^(score unit - m) with the product unrounded, while the reference point m is the largest one's rounded: half a step
+// of m apart. From |m| = 2^20 on, where that is 2^-4 and grows with m until weights overflow, a pair's products are rounded too,
+// so that the largest weighs 2^0 again; the tile's other pairs keep their bits.
+constexpr float kFar = 0x1p20f;
+template <typename V>
+__device__ __forceinline__ void round_far(V& s, float m, float& unit) {
+  if (!__any(fabsf(m) >= kFar)) return;
+  const bool far = fabsf(m) >= kFar;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] *= far ? unit : 1.0f;
+  unit = far ? 1.0f : unit;
+}
+
 // V's scales differ from block to block, so what a pair rounds to fp16 is the product of a token's weight and its block's
 // scale, relative to `vref`: at least the largest block's share (its largest weight times its scale) over 2^8 among the
 // blocks that this pair sees, and at most the largest. So the products stay at most 2^8, and each is off by 2^-11 of
@@ -283,9 +296,11 @@ constexpr float kMostScale = 0x1p126f;  // vref's, and a ratio's, largest: the r
 __device__ __forceinline__ float block_share(float top, float m, float vs) {
   return __builtin_amdgcn_exp2f(top - (m == -INFINITY ? 0.f : m)) * vs;
 }
-// Whether a page whose largest score and share are bm and vm moves the pair's reference points.
+// Whether a page whose largest score and share are bm and vm moves the pair's reference points. (Far from zero m + 8 is m, or 8
+// more: the difference is exact.)
+__device__ __forceinline__ bool higher(float bm, float m) { return bm > m + kLazy || bm - m > 2.0f * kLazy; }
 __device__ __forceinline__ bool moves(float bm, float m, float vm, float vref) {
-  return bm > m + kLazy || vm > 256.0f * vref;
+  return higher(bm, m) || vm > 256.0f * vref;
 }
 // (blocks that were never written, with scales of zero, leave it where it was)
 __device__ __forceinline__ float next_reference(float vold, float share) {

@@ -233,7 +233,7 @@ __global__ __launch_bounds__(512) void kv8_attention_wide_kernel(KvArgs a, AttnA
         const float vm = share(m);
         if (__any(moves(bm, m, vm, vref))) {
           const bool mine = moves(bm, m, vm, vref);  // a pair's own: the others of the tile keep their bits
-          const float mnew = bm > m + kLazy ? bm : m;
+          const float mnew = higher(bm, m) ? bm : m;
           const float alpha = state_weight(m, mnew), vold = alpha * vref;
           const float vnew = mine ? next_reference(vold, share(mnew)) : vref;
           const float both = mine ? vold / vnew : 1.0f;
@@ -244,6 +244,7 @@ __global__ __launch_bounds__(512) void kv8_attention_wide_kernel(KvArgs a, AttnA
           for (int i = 0; i < DT; ++i) o[i] *= both;
         }
         const float mref = m == -INFINITY ? 0.f : m;
+        round_far(st, mref, unit);
         const float ratio = blind ? 0.f : scale_ratio(vs, vref);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {

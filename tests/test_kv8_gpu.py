@@ -1108,3 +1108,49 @@ def test_attention_over_a_zeroed_pool_is_zero(gpu, kernels, stream, rows, heads,
     # weights are rounded to fp16 relative to different references: 2^-11 each of what is summed, at most the largest |v|
     _, v = t.host[0].tokens(t.table[0, :-(-n // ref.PAGE)], n)
     assert (np.abs(a - b) <= 2.0 ** -9 * np.abs(v).max()).all() and np.isfinite(a).all()
+
+
+FAR_KINDS = [KINDS[0], KINDS[2], KINDS[3], KINDS[5], KINDS[6], KINDS[7], KINDS[9], KINDS[10]]
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("scale", [1e5, 1e25])
+@pytest.mark.parametrize("rows,heads,kv,dim,n", FAR_KINDS)
+def test_attention_of_scores_far_from_zero(gpu, kernels, stream, rows, heads, kv, dim, n, scale, fmt):
+    """Scores of 30,480 times the scale, whose fp32 steps are 2^8 and more: every third key has the largest, or (negative ones) all
+    have the same, and an output is the mean of their values, within what it may be off but for the scores' part."""
+    for sign, step in ((1.0, 3), (-1.0, 1)):
+        t = Setup(kv, dim, fmt, [n], [rows], layers=1, layer=0, seed=n, behind=0)
+        k = np.zeros((n, kv, dim), np.float32)
+        k[:, :, 5] = (sign * np.where(np.arange(n) % step == 0, 240.0, 208.0))[:, None]
+        t.host[0].append(t.table, np.array([0, n]), np.arange(n), k, t.rng.standard_normal(k.shape).astype(np.float32))
+        t.device()
+        q = np.zeros((rows, heads, dim), np.float16)
+        q[:, :, 5] = 127.0
+        got = raw_attention(kernels, stream, t, heads, q.reshape(rows, -1), scale=scale).astype(np.float64)
+        kh, v = t.host[0].tokens(t.table[0, :-(-n // ref.PAGE)], n)
+        for r in range(rows):
+            m = int(t.qpos[r]) + 1
+            p = (np.arange(m) % step == 0) / -(-m // step)
+            for h in (0, heads - 1):
+                vh = v[:m, h // (heads // kv)]
+                want = p @ vh
+                bound = attention_bound(np.zeros(dim), kh[:m, 0], vh, scale, p, want)
+                assert (np.abs(got[r, h] - want) <= bound).all(), (r, h)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("rows,heads,kv,dim,n", FAR_KINDS)
+def test_attention_of_scores_far_from_zero_leaves_other_rows_alone(gpu, kernels, stream, rows, heads, kv, dim, n, fmt):
+    """Every other row's scores are about 2^28; the rows between keep the bits that they have among rows like themselves."""
+    t = Setup(kv, dim, fmt, [n], [rows], layers=1, layer=0, seed=n, behind=0)
+    k = t.rng.standard_normal((n, kv, dim)).astype(np.float32)
+    k[:, :, 5] = 240.0
+    t.host[0].append(t.table, np.array([0, n]), np.arange(n), k, t.rng.standard_normal(k.shape).astype(np.float32))
+    t.device()
+    q = t.rng.standard_normal((rows, heads, dim)).astype(np.float16)
+    q[:, :, 5] = 0.0
+    clean = raw_attention(kernels, stream, t, heads, q.reshape(rows, -1), scale=20.0)
+    q[1::2, :, 5] = 60000.0
+    got = raw_attention(kernels, stream, t, heads, q.reshape(rows, -1), scale=20.0)
+    assert np.isfinite(got.astype(np.float32)).all() and np.array_equal(got[::2], clean[::2])
