@@ -439,6 +439,28 @@ def test_a_divided_product_replays_from_a_graph(gpu):
     k.ctx.close()
 
 
+@pytest.mark.parametrize("n,k", [(64, 9000), (2560, 9216), (18432, 2560), (257, 4100), (2560, 4096), (1, 16000), (96, 0)])
+def test_the_sizing_call_holds_every_call_up_to_its_rows(gpu, n, k):
+    """A call that would have to grow the workspace is refused while its stream is captured: none is, of any epilogue."""
+    kk, s, most = Kernels(), Stream(), 300
+    wide = up(k, 128)
+    c, e = full((max(most, n), max(wide, 16)), np.uint8, 0), full((max(up(k, 512) // 512, 1), 304, 4), np.uint8, 127)
+    y = full((most, up(n, 4)), np.float32, 0)
+    m = Fp8Matrix((c, 0), max(wide, 16), (e, 0), 304)
+    kk.fp8.gemm_ws(s.handle, most, n, k)
+    g = ctypes.c_void_p()
+    check(rt().hipStreamBeginCapture(s.handle, 0), "begin")
+    try:
+        for rows in [*range(1, 20), *range(20, most, 23), 256, 257, most]:
+            for epi in Epilogue:
+                if epi != Epilogue.SwigluF16 or n % 32 == 0:
+                    kk.fp8.gemm(s.handle, m, m, (y, 0), up(n, 4), rows, n, k, epi)
+    finally:
+        check(rt().hipStreamEndCapture(s.handle, ctypes.byref(g)), "end")
+    rt().hipGraphDestroy(g)
+    kk.ctx.close()
+
+
 def test_rows_past_4_gib(gpu, kernels, stream):
     """Row strides of 2^23 bytes: the last tile's rows lie 2^32 bytes and more behind the first's."""
     from decide_amd.hip import DeviceArray
