@@ -43,7 +43,8 @@ int check_gemm(const char* op, const dh_fp8_matrix* x, const dh_fp8_matrix* w, u
   return rc;
 }
 
-// What a plan takes must fit one launch, and its partial sums the split-K workspace's ceiling.
+// What a plan takes must fit one launch. (Its partial sums are those of at most as many tiles as fit the device at once: they
+// cannot reach the split-K workspace's ceiling.)
 int plan_of(const char* op, const dh_ctx* ctx, uint32_t m, uint32_t n, uint32_t k, uint32_t epi, dh::Fp8Plan* p) {
   *p = dh::fp8_gemm_plan(m, n, k, epi, ctx->cus);
   if ((uint64_t)p->mtiles * p->ntiles * p->splits > kMaxThreads / 512)

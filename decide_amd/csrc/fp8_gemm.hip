@@ -20,8 +20,9 @@
 //     byte does not matter as long as both operands agree.
 //   * The words of X's scales of 512 columns and the tile's rows lie in LDS, for up to kSegment columns at a time, and their
 //     bytes are read with the slice.
-// Measured: 16,384 x 18,432 x 2,560 with SwiGLU 644 us (2,400 TF, matrix instructions at 76 %), 8,192 x 2,560 x 9,216 with fp32
-// outputs 315 (1,230 TF, 80 % of a large bf16 product's rate), 16 x 18,432 x 2,560 10.5 (the weight at 4.5 TB/s).
+// Measured: 16,384 x 18,432 x 2,560 with SwiGLU 639 us (2,420 TF, the matrix unit busy 66 % of the cycles), 8,192 x 2,560 x 9,216
+// with fp32 outputs 308 (1,250 TF, 71 %; a large bf16 product runs at 1,540 to 1,610 TF), 16 x 18,432 x 2,560 10.5 (the weight at
+// 4.5 TB/s).
 #include <algorithm>
 #include <cmath>
 

@@ -19,14 +19,13 @@ struct PackArgs {
   uint32_t group_inv;        // 2^21 / group, rounded up
   uint32_t slots;            // tiles are numbered below it
   uint32_t runs;             // of each kv head; 0: a workgroup a tile
-  uint32_t min_run;          // steps of a run at least
+  uint32_t min_run;          // steps (of 128 keys) of a run at least
   float scale;
 };
 
 constexpr uint32_t kPackTile = 32;       // (row, head) pairs of a tile of the kernel for few rows
 constexpr uint32_t kPackWideTile = 128;  // the same for many
 constexpr uint32_t kPackSlots = 2048;    // tiles that runs are dealt over (their steps lie in LDS)
-constexpr uint32_t kPackStep = 128;      // keys of a step
 // Steps of 32 keys that a wave of the kernel for few rows holds in LDS: 32 KB at most.
 constexpr int packed_ring(int head_dim) { return head_dim == 64 ? 3 : 256 / head_dim; }
 

@@ -29,7 +29,9 @@ __device__ __forceinline__ f16v mfma_16bit(const s8& a, const s8& b, const f16v&
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
-// rounded to nearest
+// Rounded to nearest: outputs, and the softmax's weights as the operand of P V, which is what the matrix instruction takes at
+// full rate: a weight is off by half a step of its type, as a value of V is, and sums and scores stay fp32. Against 64 bits
+// outputs are 2.5e-4 off in fp16 and 2.2e-3 in bf16 (2-norm), rounding them alone 2.1e-4 and 1.7e-3.
 template <bool BF16>
 __device__ __forceinline__ s8 pack8(const float* v) {
   if constexpr (BF16) {

@@ -407,13 +407,20 @@ hipError_t launch_packed_narrow(const PackArgs& a, uint32_t head_dim, bool bf16,
 // Runs, at the price of the deal and the merge, where narrow tiles leave half of the device idle over long sequences: one row, 32
 // heads over 8 of 128, 600 keys 10.9 us against 9.9, 4,096 keys 12 against 38; 16 over 4 of 256, 8 rows of up to 1,000 keys 24
 // against 21, one of 2,000 17 against 34; 200 rows behind 6,000 keys (100 tiles) 66 against 91; 32 over 8 of 128, 4 x 64 rows
-// behind 3,000 keys (256 tiles) 43 against 33. Single tokens make a tile a sequence, mostly empty: 64 of up to 4,096 keys
-// (64 full tiles' pairs) 61 against 65. More kv heads than half of the CUs would leave a head one run.
+// behind 3,000 keys (256 tiles) 43 against 33. More kv heads than half of the CUs would leave a head one run.
+// Single tokens make a tile a sequence, however many pairs it lacks, and the count below (as if sequences shared tiles) takes
+// many of them for few tiles and very many for a prompt. Measured, bf16, lengths of up to 4,096, wide | narrow | runs, us (* what
+// this takes): 32 heads over 8 of 128, 64 tokens 98 | 89 | 81*, 128 163 | 141* | 148, 256 295 | 270* | 290; 64 over 8, 64 tokens
+// 105 | 97* | 93, 256 304 | 281* | 277; 16 over 4 of 256, 64 tokens 159 | 100 | 77*, 256 298 | 273* | 252; 8 over 1 of 64, 256
+// 53 | 43 | 40*; 640 tokens of these 68 to 650, the three within 5 %, but for runs of 64 dims (83); 32 over 8 of 128, 288 tokens of
+// up to 200 37* | 54 | 88, of up to 1,000 100* | 114 | 156. All of 1,500: 32 over 8 of 128,
+// 64 tokens 73 | 73 | 83*, 256 269 | 272* | 301; 16 over 4 of 256, 128 tokens 129 | 136 | 149*. The keys' bytes bound these; the
+// choice costs at most 8 % where lengths differ, 15 % where they are all the same, which the host does not know.
 PackPlan packed_plan(uint32_t q_rows, uint32_t seqs, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t max_k,
                      uint32_t cus) {
   PackPlan p;
   const uint64_t pairs = (uint64_t)q_rows * (heads / kv_heads);
-  const uint64_t full = pairs / kPackTile * kv_heads;  // narrow tiles that are surely full
+  const uint64_t full = pairs / kPackTile * kv_heads;  // narrow tiles that the rows fill if sequences share them
   p.wide = full >= (head_dim == 128 ? 9ull : 11ull) * cus / 4 || (head_dim < 256 && max_k <= 1024 && full > cus);
   p.slots = (uint32_t)(pairs / (p.wide ? kPackWideTile : kPackTile) + seqs);
   const uint32_t least = head_dim == 256 ? 1024 : head_dim == 128 ? 768 : 1536;

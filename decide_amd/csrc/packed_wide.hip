@@ -8,13 +8,14 @@
 //     pair are in its two lanes, and the weights are, as they are, the operand of P^T: eight a lane for 16 keys, 4 h + j and
 //     8 + 4 h + j. V's operand is to hold the same keys for each dim: two transposing reads of four rows of V each.
 //   * K and V go into LDS by DMA, two blocks in turn, their chunks swizzled (packed_device.h). Two workgroups share a CU, and so
-//     two waves a SIMD, which need not be in step: 8,192 rows of 32 heads over 8 of 128 dims 522 us (1,050 TF); when it took
+//     two waves a SIMD, which need not be in step: 8,192 rows of 32 heads over 8 of 128 dims 531 us (1,040 TF); when it took
 //     585, eight waves in one workgroup on a ring of four blocks took 611, and with the two of a SIMD kept half a block apart
-//     614; three workgroups with blocks of 32 keys 620. Matrix and vector instructions (the softmax) bound it, 45 and 42 %
-//     of the cycles, and they hardly overlap.
+//     614; three workgroups with blocks of 32 keys 620. Matrix and vector instructions (the softmax) bound it, the matrix unit
+//     busy 58 % of the cycles and vector instructions issued in 53 %.
 //   * The softmax's reference point moves only where a score exceeds it by 2^8, so O is rarely rescaled.
-//   * Of 256 dims, 24 prompts of up to 2,307 rows and 16 heads over 4, 19.5 k rows in all, with gates: 395 us; there the bytes of
-//     Q, y and the gates alone are 161 us.
+//   * Of 256 dims, 24 prompts of up to 2,307 rows and 16 heads over 4, 21,864 rows in all, with gates: 375 us; there the bytes of
+//     Q, y and the gates alone are 151 us. The matrix unit is busy 38 % of the cycles, and waves wait 32 %; this was not tried
+//     with other blocks or tiles.
 //   * Keys past the sequence's end are its last one again, masked: another sequence's values are never touched.
 #include "packed_device.h"
 

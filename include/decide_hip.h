@@ -733,7 +733,8 @@ int dh_fp8_quant_blocks(dh_ctx* ctx, void* stream, const void* w, uint32_t ldw, 
  * fp32; with fp16 outputs (SwiGLU among them) the products of each eight
  * neighbouring columns are first added by the matrix instruction, which cuts
  * what lies more than 13 bits below the largest of them (2^-13 of the largest
- * product a term at most, a thirtieth of an fp16 rounding on ordinary data).
+ * product a term at most; beside an fp16 rounding a fourteenth of its error on
+ * normal data, a fifth where columns differ by factors of e).
  * With fp32 outputs values are held as bfloat16 first: exactly where the byte
  * of their scale is 3 .. 246, whatever the code; beyond, what is past
  * bfloat16's largest number counts as infinite and what is no multiple of its
